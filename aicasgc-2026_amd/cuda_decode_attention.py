@@ -15,6 +15,9 @@ LSE) partials either by the last-arriving workgroup (``*_fused`` and
 ``*_cta_*`` names) or by a separate merge launch (``decode_attn_v4_splitkv``).
 ``split_k`` is honoured as a minimum split count; the kernel may use more
 splits to fill 256 CUs (results do not depend on the split count).
+
+``attn_fp8_kv_cache`` has no counterpart there: attention over the 8-bit cache of
+``cuda_decode_small_ops.new_kv_cache_fp8``.
 """
 
 from __future__ import annotations
@@ -23,9 +26,11 @@ from functools import lru_cache
 
 import torch
 
+from cuda_decode_small_ops import _half_rows, _kv_fp8_args, _positions, _strided_heads
 from qwen3vl_hip import _lib
 
 _WS_KEY = "_qd_attention_ws"
+_FP8_WS_KEY = "_qd_attention_fp8_ws"
 
 
 def _load_ext():
@@ -212,3 +217,51 @@ def grouped_prefix_cachepos_splitkv_qhead(q, k, v, scaling, num_key_value_groups
     if split_k <= 1:
         return None
     return _run_fused(q, k, v, scaling, num_key_value_groups, cache_position, split_k, workspace)
+
+
+@lru_cache(maxsize=1024)
+def _fp8_ws_bytes(b: int, sq: int, hq: int, hkv: int, t: int, window: int, sinks: int) -> int:
+    return int(_load_ext().qd_attention_fp8_workspace_bytes(b, sq, hq, hkv, t, window, sinks))
+
+
+def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0, sinks: int = 0,
+                      workspace: dict | None = None):
+    """Causal attention of Sq query tokens per sequence over the 8-bit KV cache
+    (``cuda_decode_small_ops.KVCacheFP8``): q [B, Hq, Sq, 128] fp16 at any strides, the
+    result [B, Sq, Hq, 128] fp16.
+
+    Query token i of sequence b stands at row p = cache_position[b] + i (int64 [B])
+    and sees the rows t <= p below the capacity; with ``window`` > 0 only those with
+    t > p - window or t < ``sinks``.  A token that sees no row gets zeros.  The new
+    tokens' own rows must be in the cache (``fused_q_rope_kv_cache_update_fp8``).
+    Head h reads kv head h // (Hq / Hkv).  ``scaling`` must be positive.
+
+    ``workspace`` keeps the kernel's scratch memory between calls (it holds nothing
+    from one call to the next, so it needs no clearing, but two calls in flight at
+    once must not share it).  Unlike the other entry points, inputs outside what the
+    kernel supports raise RuntimeError: there is no other path over this cache."""
+    name = "attn_fp8_kv_cache"
+    dev = _half_rows(name, q)
+    if q.ndim != 4 or q.shape[3] != 128:
+        raise RuntimeError(f"{name}: q must be [B, Hq, Sq, 128]")
+    b, h, t, where = _kv_fp8_args(name, cache, dev)
+    bq, hq, sq = q.shape[:3]
+    if bq != b or hq < h or hq % h:
+        raise RuntimeError(f"{name}: q needs the cache's batch and a multiple of its kv heads")
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"{name}: window and sinks must not be negative")
+    cp = _positions(name, cache_position, b, dev)
+    qi = _strided_heads(q, 8)
+    out = torch.empty((b, sq, hq, 128), dtype=q.dtype, device=dev)
+    need = _fp8_ws_bytes(b, sq, hq, h, t, window, sinks)
+    ws = None
+    if need:
+        ws = workspace.get(_FP8_WS_KEY) if workspace is not None else None
+        if ws is None or ws.numel() < need or ws.device != dev:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            if workspace is not None:
+                workspace[_FP8_WS_KEY] = ws
+    _lib.call_on(dev, "qd_attention_fp8", qi.data_ptr(), *qi.stride()[:3], *where, cp.data_ptr(), float(scaling), window,
+                 sinks, out.data_ptr(), b, sq, hq, h, _lib.ptr(ws), need)
+    return out

@@ -3,3 +3,6 @@
 
 from cuda_decode_gemv_ops import *  # noqa: F401,F403
 from cuda_decode_gemv_ops import __all__  # noqa: F401
+
+# beside the reference's names (its __all__), not among them
+from cuda_decode_gemv_ops.blocked import block_matmul_fp8  # noqa: F401

@@ -87,6 +87,17 @@ _SIGS = {
     "qd_batch_gemv": (c_int, [P, c_long, P, c_float, P, c_long, c_long, c_long, c_long, P, c_long, P, c_long, c_int,
                               c_int, P, ctypes.c_size_t, P]),
     "qd_decode_set_state": (c_int, [P, P, P, P, POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_int, P]),
+    "qd_quantize_fp8": (c_int, [P, c_long, P, P, c_long, c_long, c_int, P]),
+    "qd_silu_mul_fp8": (c_int, [P, c_long, P, c_long, P, P, c_long, c_long, P]),
+    "qd_add_rmsnorm_fp8": (c_int, [P, c_long, P, c_long, P, P, P, P, c_long, c_long, c_float, P]),
+    "qd_block_matmul_fp8": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, P]),
+    "qd_q_rope_kv_update_fp8": (c_int, [P, c_long, c_long, c_long, P, c_long, c_long, c_long, P, c_long, c_long, c_long,
+                                        P, P, c_float, P, P, P, P, P, P, P, c_long, c_long, c_long, c_long, c_int, P,
+                                        c_int, c_int, c_int, c_int, P]),
+    "qd_kv_read_fp8": (c_int, [P, P, P, P, c_long, c_long, c_long, c_long, c_int, P, P, c_int, c_int, c_int, P]),
+    "qd_attention_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "qd_attention_fp8": (c_int, [P, c_long, c_long, c_long, P, P, P, P, c_long, c_long, c_long, c_long, c_int, P, c_float,
+                                 c_int, c_int, P, c_int, c_int, c_int, c_int, P, c_size_t, P]),
     "qd_decode_advance_batch": (c_int, [P, P, P, P, P, c_int, c_int, P]),
 }
 
@@ -134,6 +145,17 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device``'s current stream as the last argument, whatever the
+    current device is (a kernel launches on the current device only)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+    else:
+        with torch.cuda.device(device):
+            check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+
+
 class ModelDesc(ctypes.Structure):
     pass
 
@@ -164,5 +186,5 @@ ModelDesc._fields_ = [
     ("batch_tiled_weights", c_int),
 ]
 
-__all__ = ["lib", "check", "ptr", "stream", "call", "QD_F16", "QD_F32", "ModelDesc", "LayerDesc", "EXPORTED",
+__all__ = ["lib", "check", "ptr", "stream", "call", "call_on", "QD_F16", "QD_F32", "ModelDesc", "LayerDesc", "EXPORTED",
            "LIB_PATH", "c_int64"]

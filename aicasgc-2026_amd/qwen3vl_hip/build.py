@@ -21,7 +21,8 @@ LIB_NAME = "libqwen3vl_decode.so"
 LIB_PATH = PKG_ROOT / LIB_NAME
 TRACE_LIB_PATH = PKG_ROOT / "libqwen3vl_decode_trace.so"   # same sources with -DQD_TRACE
 SOURCES = ["qd_gemv.hip", "qd_attention.hip", "qd_small_ops.hip", "qd_persistent.hip", "qd_batch.hip", "qd_prefill.hip",
-           "qd_capi.hip"]
+           "qd_fp8.hip", "qd_fp8_gemm.hip", "qd_fp8_attention.hip",
+           "qd_fp8_capi.hip", "qd_capi.hip"]
 ARCH = os.environ.get("QD_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -263,6 +263,83 @@ int qd_attention_merge(const float* o_part, const float* lse, void* out, int out
  * (32 splits from T = 3969 on: 256 workgroups at 8 kv heads). */
 int qd_attention_default_splits(int T);
 
+/* ------------------------------------------------------------------ 8-bit operators
+ *
+ * No counterpart in the reference, whose weights and cache are fp16.  Values are
+ * e4m3 (OCP), scales powers of two stored as E8M0 bytes, 2^(byte - 127), one per
+ * block.  A block's exponent is the least e with amax <= 448 * 2^e, amax over its
+ * finite values (e >= -126; in the cache e >= -32); NaN and infinities are
+ * stored as NaN.  A value is rounded once, to nearest even, from fp32.  Inputs
+ * and norm weights are fp16. */
+
+/* q = x in 8 bits; x [rows][cols] with row stride ldx.  block_rows 1: scale
+ * [rows][ceil(cols / 128)], one per row and 128 columns.  block_rows 128: scale
+ * [ceil(rows / 128)][ceil(cols / 128)], one per 128 x 128 block (weights). */
+int qd_quantize_fp8(const void* x, long ldx, void* q, void* scale, long rows, long cols, int block_rows, void* stream);
+
+/* q = silu(gate) * up in 8 bits, a scale per row and 128 columns; gate and up
+ * [rows][cols] with row strides ld_gate, ld_up. */
+int qd_silu_mul_fp8(const void* gate, long ld_gate, const void* up, long ld_up, void* q, void* scale, long rows,
+                    long cols, void* stream);
+
+/* q = rmsnorm(residual + x) * weight in 8 bits, a scale per row and 128 columns;
+ * out_sum (fp16, may be NULL) = residual + x.  residual NULL: rmsnorm(x).  The
+ * norm is taken of the fp32 sum.  x and residual have row strides ldx and
+ * ld_residual; q and out_sum are contiguous. */
+int qd_add_rmsnorm_fp8(const void* residual, long ld_residual, const void* x, long ldx, const void* weight,
+                       void* out_sum, void* q, void* scale, long rows, long cols, float eps, void* stream);
+
+/* y[M][N] = x[M][K] W[N][K]^T of 8-bit operands: x_scale [M][ceil(K / 128)],
+ * w_scale [ceil(N / 128)][ceil(K / 128)], y in y_dtype.  K a multiple of 16,
+ * at most 2^23; M <= 2^20, N <= 2^24; x, w and y 16-byte aligned; products of two
+ * scales within fp32's range.  Sums are fp32; of fp16 results for more than 64 rows
+ * those of each 8 products at neighbouring k (8 j .. 8 j + 7) keep what is above
+ * 2^-13 of the largest of them. */
+int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const void* w_scale, void* y, int y_dtype,
+                        int M, int N, int K, void* stream);
+
+/* The 8-bit cache of B sequences and Hkv heads, T rows each (a multiple of 64):
+ * k_cache [T][128] per head, v_cache [T / 64][128][64] per head (each 64-row block
+ * transposed), batch and head strides stride_b and stride_h in bytes for both;
+ * k_scale and v_scale [T / 64] per head, strides scale_stride_b and
+ * scale_stride_h.  Heads are contiguous and 16-byte aligned.
+ *
+ * qd_q_rope_kv_update_fp8: RMSNorm (head_dim 128) + rotate-half RoPE of q and k for
+ * S new tokens of each sequence, cos / sin fp16 [B][S][128]; q_out fp16
+ * [B][S][Hq][128]; K_rot and V to the rows cache_position[b] + i (int64 [B]; rows
+ * outside [0, T) are not written).  q, k, v have batch, token and head strides in
+ * elements.  A block that holds rows before cache_position[b] keeps its scale or
+ * takes a larger one, and then those rows are scaled down in place (exact but for
+ * values that become subnormal); rows behind the last written one keep their
+ * bytes, but not their meaning.  Hq is 1 to 64 times Hkv.
+ *
+ * qd_kv_read_fp8: rows [0, rows) in fp16, k_out and v_out [B][Hkv][rows][128]. */
+int qd_q_rope_kv_update_fp8(const void* q, long q_sb, long q_ss, long q_sh, const void* k, long k_sb, long k_ss,
+                            long k_sh, const void* v, long v_sb, long v_ss, long v_sh, const void* q_weight,
+                            const void* k_weight, float eps, const void* cos, const void* sin, void* q_out,
+                            void* k_cache, void* v_cache, void* k_scale, void* v_scale, long stride_b, long stride_h,
+                            long scale_stride_b, long scale_stride_h, int T, const int64_t* cache_position, int B,
+                            int S, int Hq, int Hkv, void* stream);
+int qd_kv_read_fp8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, long stride_b,
+                   long stride_h, long scale_stride_b, long scale_stride_h, int T, void* k_out, void* v_out, int B,
+                   int Hkv, int rows, void* stream);
+
+/* Causal attention of Sq query tokens per sequence over the 8-bit cache:
+ *   out[b][i][h] = softmax over the visible rows t of scale q_h.k_t, times v_t
+ * for q head h on kv head h / (Hq / Hkv); query token i stands at
+ * p = cache_position[b] + i and sees the rows t <= p, t < T and, with window > 0,
+ * t > p - window or t < sinks.  No visible row: zeros.  q fp16 with batch, head and
+ * token strides in elements (multiples of 8); out fp16 [B][Sq][Hq][128];
+ * scale > 0.  A NaN in a row that a token does not see has no part in its result.
+ * workspace: qd_attention_fp8_workspace_bytes(...) bytes, 16-byte aligned (NULL
+ * where that is 0); it holds nothing between calls, but two calls in flight must
+ * not share it. */
+size_t qd_attention_fp8_workspace_bytes(int B, int Sq, int Hq, int Hkv, int T, int window, int sinks);
+int qd_attention_fp8(const void* q, long q_sb, long q_sh, long q_ss, const void* k_cache, const void* v_cache,
+                     const void* k_scale, const void* v_scale, long stride_b, long stride_h, long scale_stride_b,
+                     long scale_stride_h, int T, const int64_t* cache_position, float scale, int window, int sinks,
+                     void* out, int B, int Sq, int Hq, int Hkv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ decode step */
 
 /* One decoder layer's weights (fused layout of optimized_layer.py:60-84). */
