@@ -156,8 +156,8 @@ int qd_attention_fp8(const void* q, long q_sb, long q_sh, long q_ss, const void*
   QD_TRY(check_cache(a.c, const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<void*>(k_scale),
                      const_cast<void*>(v_scale), stride_b, stride_h, scale_stride_b, scale_stride_h, T, B, Hkv));
   QD_REQUIRE(Hq >= Hkv && Hq % Hkv == 0, QD_ERR_SHAPE, "Hq must be a multiple of Hkv (Hq=%d Hkv=%d)", Hq, Hkv);
-  QD_REQUIRE(Sq >= 0 && (long)Sq * (Hq / Hkv) <= 16L * 65535, QD_ERR_SHAPE,
-             "Sq * Hq / Hkv must be at most %ld (Sq=%d)", 16L * 65535, Sq);
+  QD_REQUIRE(Sq >= 0 && (long)Sq * (Hq / Hkv) <= (1L << 22) && (long)B * Hkv * ((long)Sq * (Hq / Hkv) / 64 + 1) < (1L << 23),
+             QD_ERR_SHAPE, "too many query rows (B=%d Sq=%d Hq=%d)", B, Sq, Hq);
   QD_REQUIRE(window >= 0 && sinks >= 0, QD_ERR_ARG, "window and sinks must not be negative (%d, %d)", window, sinks);
   QD_REQUIRE(scale > 0.f && scale <= 3.402823466e38f, QD_ERR_ARG, "scale must be positive and finite (%g)", (double)scale);
   if (B == 0 || Sq == 0) return QD_OK;

@@ -26,7 +26,7 @@ from functools import lru_cache
 
 import torch
 
-from cuda_decode_small_ops import _half_rows, _kv_fp8_args, _positions, _strided_heads
+from cuda_decode_small_ops import _half_gpu, _kv_fp8_args, _positions, _strided_heads
 from qwen3vl_hip import _lib
 
 _WS_KEY = "_qd_attention_ws"
@@ -241,27 +241,26 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
     once must not share it).  Unlike the other entry points, inputs outside what the
     kernel supports raise RuntimeError: there is no other path over this cache."""
     name = "attn_fp8_kv_cache"
-    dev = _half_rows(name, q)
-    if q.ndim != 4 or q.shape[3] != 128:
+    dev = _half_gpu(name, q)
+    if q.ndim != 4:
         raise RuntimeError(f"{name}: q must be [B, Hq, Sq, 128]")
     b, h, t, where = _kv_fp8_args(name, cache, dev)
-    bq, hq, sq = q.shape[:3]
-    if bq != b or hq < h or hq % h:
-        raise RuntimeError(f"{name}: q needs the cache's batch and a multiple of its kv heads")
-    window, sinks = int(window), int(sinks)
+    bq, hq, sq, d = q.shape
+    if d != 128 or bq != b or hq < h or hq % h:
+        raise RuntimeError(f"{name}: q must be [B, Hq, Sq, 128] with the cache's batch and a multiple of its kv heads")
     if window < 0 or sinks < 0:
         raise RuntimeError(f"{name}: window and sinks must not be negative")
     cp = _positions(name, cache_position, b, dev)
     qi = _strided_heads(q, 8)
-    out = torch.empty((b, sq, hq, 128), dtype=q.dtype, device=dev)
+    out = q.new_empty((b, sq, hq, 128))
     need = _fp8_ws_bytes(b, sq, hq, h, t, window, sinks)
     ws = None
     if need:
         ws = workspace.get(_FP8_WS_KEY) if workspace is not None else None
-        if ws is None or ws.numel() < need or ws.device != dev:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if ws is None or ws.numel() < need or ws.get_device() != dev:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             if workspace is not None:
                 workspace[_FP8_WS_KEY] = ws
-    _lib.call_on(dev, "qd_attention_fp8", qi.data_ptr(), *qi.stride()[:3], *where, cp.data_ptr(), float(scaling), window,
-                 sinks, out.data_ptr(), b, sq, hq, h, _lib.ptr(ws), need)
+    _lib.call_on(dev, _lib.entry("qd_attention_fp8"), qi.data_ptr(), *qi.stride()[:3], *where, cp.data_ptr(), scaling, window,
+                 sinks, out.data_ptr(), b, sq, hq, h, None if ws is None else ws.data_ptr(), need)
     return out

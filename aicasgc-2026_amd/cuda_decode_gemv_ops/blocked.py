@@ -19,24 +19,31 @@ def block_matmul_fp8(x, x_scale, weight, weight_scale, out_dtype: torch.dtype = 
     [ceil(N / 128), ceil(K / 128)] (``quantize_fp8(w, block_rows=128)``); K a
     multiple of 16.  From one row (a decode token) to thousands (a prompt)."""
     name = "block_matmul_fp8"
-    dev = x.device
-    if dev.type != "cuda" or x.dtype != _F8 or weight.dtype != _F8 or x_scale.dtype != _E8 or weight_scale.dtype != _E8:
-        raise RuntimeError(f"{name}: x and weight must be float8_e4m3fn and the scales float8_e8m0fnu on the GPU")
-    if weight.device != dev or x_scale.device != dev or weight_scale.device != dev:
-        raise RuntimeError(f"{name}: tensors on different devices")
+    dev = x.get_device()
+    if (x.dtype is not _F8 or weight.dtype is not _F8 or x_scale.dtype is not _E8 or weight_scale.dtype is not _E8
+            or dev < 0 or weight.get_device() != dev or x_scale.get_device() != dev or weight_scale.get_device() != dev):
+        raise RuntimeError(f"{name}: x and weight must be float8_e4m3fn and the scales float8_e8m0fnu, all on one GPU")
+    lead = x.shape[:-1]
     if weight.ndim != 2 or x.ndim < 1:
         raise RuntimeError(f"{name}: weight must be [N, K] and x [..., K]")
     n, k = weight.shape
     kb = (k + 127) // 128
-    if x.shape[-1] != k or x_scale.shape != (*x.shape[:-1], kb) or weight_scale.shape != ((n + 127) // 128, kb):
+    if x.shape[-1] != k or x_scale.shape != (*lead, kb) or weight_scale.shape != ((n + 127) // 128, kb):
         raise RuntimeError(f"{name}: need x [..., {k}] with scales [..., {kb}] and weight scales [{(n + 127) // 128}, {kb}]")
     if n < 1 or k < 16 or k % 16:
         raise RuntimeError(f"{name}: K must be a positive multiple of 16 and N positive")
     code = _OUT.get(out_dtype)
     if code is None:
         raise RuntimeError(f"{name}: out_dtype must be float16 or float32")
-    xi, xs, w, ws = x.contiguous(), x_scale.contiguous(), weight.contiguous(), weight_scale.contiguous()
-    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=dev)
-    _lib.call_on(dev, "qd_block_matmul_fp8", xi.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), code,
-                 x.numel() // k, n, k)
+    xi, xs, w, ws = _aligned(x), x_scale.contiguous(), _aligned(weight), weight_scale.contiguous()
+    y = x.new_empty((*lead, n), dtype=out_dtype)
+    _lib.call_on(dev, _lib.entry("qd_block_matmul_fp8"), xi.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                 y.data_ptr(), code, x.numel() // k, n, k)
     return y
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy of it at a 16-byte aligned address."""
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()

@@ -174,15 +174,13 @@ FP8_COLS = 128       # columns (and, of a weight, rows) per scale
 KV_FP8_BLOCK = 64    # cache rows per scale
 
 
-def _half_rows(name: str, *ts) -> torch.device:
-    """The device of fp16 GPU tensors that all lie on it."""
-    d = ts[0].device
+def _half_gpu(name: str, *ts) -> int:
+    """The GPU that holds the fp16 tensors ``ts``, all of them."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t.device.type != "cuda" or t.dtype != torch.float16:
-            raise RuntimeError(f"{name}: every tensor must be fp16 on the GPU")
-        if t.device != d:
-            raise RuntimeError(f"{name}: tensors on different devices ({t.device}, {d})")
-    return d
+        if t.dtype is not torch.float16 or t.get_device() != dev or dev < 0:
+            raise RuntimeError(f"{name}: every tensor must be fp16 on the GPU, on one device")
+    return dev
 
 
 def _as_rows(t: torch.Tensor):
@@ -208,71 +206,74 @@ def _as_rows(t: torch.Tensor):
 
 def _quantized_like(name: str, x: torch.Tensor):
     """Empty e4m3 values of x's shape, their scales, and (rows, cols)."""
-    if x.ndim < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    if cols < 1:
         raise RuntimeError(f"{name}: rows must have at least one column")
-    cols = x.shape[-1]
-    q = torch.empty(x.shape, dtype=_F8, device=x.device)
-    scale = torch.empty((*x.shape[:-1], (cols + FP8_COLS - 1) // FP8_COLS), dtype=_E8, device=x.device)
-    return q, scale, x.numel() // cols, cols
+    blocks = (cols + FP8_COLS - 1) // FP8_COLS
+    return (x.new_empty(shape, dtype=_F8), x.new_empty((*shape[:-1], blocks), dtype=_E8), x.numel() // cols, cols)
 
 
 def quantize_fp8(x, block_rows: int = 1):
     """e4m3 values and scales of x [..., cols]: a scale per row and 128 columns, or,
     with ``block_rows=128``, per 128 x 128 block of a matrix [rows, cols] (a weight)."""
-    dev = _half_rows("quantize_fp8", x)
+    dev = _half_gpu("quantize_fp8", x)
     if block_rows not in (1, FP8_COLS):
         raise RuntimeError("quantize_fp8: block_rows must be 1 or 128")
     if block_rows != 1 and x.ndim != 2:
         raise RuntimeError("quantize_fp8: blocks of 128 rows need a matrix [rows, cols]")
     q, scale, rows, cols = _quantized_like("quantize_fp8", x)
     if block_rows != 1:
-        scale = torch.empty(((rows + FP8_COLS - 1) // FP8_COLS, scale.shape[1]), dtype=_E8, device=dev)
+        scale = x.new_empty(((rows + FP8_COLS - 1) // FP8_COLS, scale.shape[1]), dtype=_E8)
     xi, ld = _as_rows(x)
-    _lib.call_on(dev, "qd_quantize_fp8", xi.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, cols, block_rows)
+    _lib.call_on(dev, _lib.entry("qd_quantize_fp8"), xi.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, cols,
+                 block_rows)
     return q, scale
 
 
 def fused_silu_mul_fp8(gate, up):
     """silu(gate) * up in 8 bits: (values, scales).  gate and up [..., cols] may be the
     two halves of one product's output (rows at any stride)."""
-    dev = _half_rows("fused_silu_mul_fp8", gate, up)
+    dev = _half_gpu("fused_silu_mul_fp8", gate, up)
     if gate.shape != up.shape:
         raise RuntimeError("fused_silu_mul_fp8: gate and up shapes differ")
     q, scale, rows, cols = _quantized_like("fused_silu_mul_fp8", gate)
     g, ldg = _as_rows(gate)
     u, ldu = _as_rows(up)
-    _lib.call_on(dev, "qd_silu_mul_fp8", g.data_ptr(), ldg, u.data_ptr(), ldu, q.data_ptr(), scale.data_ptr(), rows, cols)
+    _lib.call_on(dev, _lib.entry("qd_silu_mul_fp8"), g.data_ptr(), ldg, u.data_ptr(), ldu, q.data_ptr(), scale.data_ptr(),
+                 rows, cols)
     return q, scale
 
 
-def _norm_fp8(name, residual, x, weight, eps):
+def _norm_fp8(name, dev, residual, x, weight, eps):
     q, scale, rows, cols = _quantized_like(name, x)
     if weight.numel() != cols:
         raise RuntimeError(f"{name}: weight length differs from the last dimension")
     xi, ld = _as_rows(x)
     wc = weight.contiguous()
-    ri, ldr, total = None, 0, None
+    ri, ldr, total, r_ptr, t_ptr = None, 0, None, None, None
     if residual is not None:
         ri, ldr = _as_rows(residual)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _lib.call_on(x.device, "qd_add_rmsnorm_fp8", _lib.ptr(ri), ldr, xi.data_ptr(), ld, wc.data_ptr(), _lib.ptr(total),
-                 q.data_ptr(), scale.data_ptr(), rows, cols, float(eps))
+        total = x.new_empty(x.shape)
+        r_ptr, t_ptr = ri.data_ptr(), total.data_ptr()
+    _lib.call_on(dev, _lib.entry("qd_add_rmsnorm_fp8"), r_ptr, ldr, xi.data_ptr(), ld, wc.data_ptr(), t_ptr, q.data_ptr(),
+                 scale.data_ptr(), rows, cols, eps)
     return total, q, scale
 
 
 def fused_add_rms_norm_fp8(residual, x, weight, eps: float):
     """(residual + x in fp16, rmsnorm(residual + x) * weight in 8 bits: values, scales).
     The norm is taken of the unrounded sum, as ``fused_add_rms_norm`` does."""
-    _half_rows("fused_add_rms_norm_fp8", residual, x, weight)
+    dev = _half_gpu("fused_add_rms_norm_fp8", residual, x, weight)
     if residual.shape != x.shape:
         raise RuntimeError("fused_add_rms_norm_fp8: residual and x shapes differ")
-    return _norm_fp8("fused_add_rms_norm_fp8", residual, x, weight, eps)
+    return _norm_fp8("fused_add_rms_norm_fp8", dev, residual, x, weight, eps)
 
 
 def rms_norm_fp8(x, weight, eps: float):
     """rmsnorm(x) * weight over the last dim in 8 bits: (values, scales)."""
-    _half_rows("rms_norm_fp8", x, weight)
-    return _norm_fp8("rms_norm_fp8", None, x, weight, eps)[1:]
+    dev = _half_gpu("rms_norm_fp8", x, weight)
+    return _norm_fp8("rms_norm_fp8", dev, None, x, weight, eps)[1:]
 
 
 class KVCacheFP8(NamedTuple):
@@ -300,38 +301,43 @@ def new_kv_cache_fp8(batch: int, kv_heads: int, capacity: int, device="cuda") ->
                       zeros(_E8, batch, kv_heads, nb), zeros(_E8, batch, kv_heads, nb))
 
 
-def _kv_fp8_args(name: str, cache, device):
-    """(B, Hkv, T, the C entries' cache arguments) of a valid cache on ``device``."""
+def _kv_fp8_args(name: str, cache, dev: int):
+    """(B, Hkv, T, the C entries' cache arguments) of a valid cache on GPU ``dev``."""
     k, v, ks, vs = cache
-    if (k.dtype != _F8 or v.dtype != _F8 or ks.dtype != _E8 or vs.dtype != _E8 or k.ndim != 4 or v.ndim != 5
-            or k.device != device or v.device != device or ks.device != device or vs.device != device):
+    if (k.dtype is not _F8 or v.dtype is not _F8 or ks.dtype is not _E8 or vs.dtype is not _E8 or k.ndim != 4
+            or k.get_device() != dev or v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev):
         raise RuntimeError(f"{name}: cache must be a KVCacheFP8 on the inputs' device")
     b, h, t, d = k.shape
     nb = t // KV_FP8_BLOCK
-    if (d != 128 or t != nb * KV_FP8_BLOCK or v.shape != (b, h, nb, 128, KV_FP8_BLOCK) or ks.shape != (b, h, nb)
-            or vs.shape != (b, h, nb)):
+    shape = ks.shape
+    if (d != 128 or t != nb * KV_FP8_BLOCK or shape != (b, h, nb) or vs.shape != shape
+            or v.shape != (b, h, nb, 128, KV_FP8_BLOCK)):
         raise RuntimeError(f"{name}: cache shapes must be k [B, Hkv, T, 128], v [B, Hkv, T / 64, 128, 64] and scales "
                            "[B, Hkv, T / 64]")
-    kt, vt, kst, vst = k.stride(), v.stride(), ks.stride(), vs.stride()
-    if (kt[2:] != (128, 1) or vt[3:] != (KV_FP8_BLOCK, 1) or (nb > 1 and (vt[2] != 128 * KV_FP8_BLOCK or kst[2] != 1 or vst[2] != 1))
-            or (b > 1 and (kt[0] != vt[0] or kst[0] != vst[0])) or (h > 1 and (kt[1] != vt[1] or kst[1] != vst[1]))):
-        raise RuntimeError(f"{name}: a head of the cache must be contiguous, k and v at the same strides")
-    return b, h, t, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt[0], kt[1], kst[0], kst[1], t)
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3, v4 = v.stride()
+    s0, s1, s2 = ks.stride()
+    if (k2 != 128 or k3 != 1 or v3 != KV_FP8_BLOCK or v4 != 1
+            or (nb > 1 and (v2 != 128 * KV_FP8_BLOCK or s2 != 1)) or (b > 1 and k0 != v0) or (h > 1 and k1 != v1)
+            or vs.stride() != (s0, s1, s2)):
+        raise RuntimeError(f"{name}: a head of the cache must be contiguous, k and v (and their scales) at the same strides")
+    return b, h, t, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k0, k1, s0, s1, t)
 
 
-def _positions(name: str, cache_position, b: int, device) -> torch.Tensor:
-    if cache_position.dtype != torch.long or cache_position.device != device or cache_position.shape != (b,):
+def _positions(name: str, cache_position, b: int, dev: int) -> torch.Tensor:
+    if cache_position.dtype is not torch.int64 or cache_position.get_device() != dev or cache_position.shape != (b,):
         raise RuntimeError(f"{name}: cache_position must be int64 [{b}] on the inputs' device")
-    return cache_position.contiguous()
+    return cache_position if cache_position.is_contiguous() else cache_position.contiguous()
 
 
 def _strided_heads(t: torch.Tensor, multiple: int) -> torch.Tensor:
-    """t [B, S, H, 128] (any order of the first three) itself where its heads can be
+    """t [.., .., .., 128] (any order of the first three) itself where its heads can be
     read in place: contiguous, at strides and an address of whole ``multiple``s."""
-    st = t.stride()
-    if st[3] == 1 and not ((st[0] | st[1] | st[2]) % multiple) and not t.data_ptr() % (2 * multiple):
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and not (s0 | s1 | s2) % multiple and not t.data_ptr() % (2 * multiple):
         return t
-    return t.contiguous()
+    t = t.contiguous()
+    return t if not t.data_ptr() % (2 * multiple) else t.clone()
 
 
 def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, cos, sin, cache: KVCacheFP8,
@@ -347,13 +353,13 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
     not written here are no longer the sequence's: a block's scale follows the
     rows up to the last one written."""
     name = "fused_q_rope_kv_cache_update_fp8"
-    dev = _half_rows(name, q, k, v, q_weight, k_weight, cos, sin)
-    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != 128 or k.shape[3] != 128:
+    dev = _half_gpu(name, q, k, v, q_weight, k_weight, cos, sin)
+    if q.ndim != 4 or k.ndim != 4:
         raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128]")
+    bs, s, hq, d = q.shape
     b, h, t, where = _kv_fp8_args(name, cache, dev)
-    bs, s, hq = q.shape[:3]
-    if bs != b or k.shape[2] != h:
-        raise RuntimeError(f"{name}: cache and k have different batches or kv head counts")
+    if d != 128 or k.shape != (bs, s, h, 128) or v.shape != (bs, s, h, 128) or bs != b:
+        raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128], with the cache's B and Hkv")
     if hq % h or not h <= hq <= 64 * h:
         raise RuntimeError(f"{name}: q heads must be 1 to 64 times the kv heads")
     if q_weight.numel() != 128 or k_weight.numel() != 128:
@@ -363,22 +369,22 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
     cp = _positions(name, cache_position, b, dev)
     qi, ki, vi = _strided_heads(q, 4), _strided_heads(k, 4), _strided_heads(v, 4)
     qw, kw, cs, sn = q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous()
-    out = torch.empty((b, s, hq, 128), dtype=q.dtype, device=dev)
-    _lib.call_on(dev, "qd_q_rope_kv_update_fp8", qi.data_ptr(), *qi.stride()[:3], ki.data_ptr(), *ki.stride()[:3],
-                 vi.data_ptr(), *vi.stride()[:3], qw.data_ptr(), kw.data_ptr(), float(eps), cs.data_ptr(), sn.data_ptr(),
+    out = q.new_empty((b, s, hq, 128))
+    _lib.call_on(dev, _lib.entry("qd_q_rope_kv_update_fp8"), qi.data_ptr(), *qi.stride()[:3], ki.data_ptr(), *ki.stride()[:3],
+                 vi.data_ptr(), *vi.stride()[:3], qw.data_ptr(), kw.data_ptr(), eps, cs.data_ptr(), sn.data_ptr(),
                  out.data_ptr(), *where, cp.data_ptr(), b, s, hq, h)
     return out
 
 
 def read_kv_cache_fp8(cache: KVCacheFP8, rows: int):
     """The first ``rows`` rows of every sequence in fp16: (k, v), each [B, Hkv, rows, 128]."""
-    dev = cache[0].device
-    if dev.type != "cuda":
+    dev = cache[0].get_device()
+    if dev < 0:
         raise RuntimeError("read_kv_cache_fp8: the cache must be on the GPU")
     b, h, t, where = _kv_fp8_args("read_kv_cache_fp8", cache, dev)
     if not 0 <= rows <= t:
         raise RuntimeError(f"read_kv_cache_fp8: rows must lie in [0, {t}]")
-    k = torch.empty((b, h, rows, 128), dtype=torch.float16, device=dev)
+    k = torch.empty((b, h, rows, 128), dtype=torch.float16, device=cache[0].device)
     v = torch.empty_like(k)
-    _lib.call_on(dev, "qd_kv_read_fp8", *where, k.data_ptr(), v.data_ptr(), b, h, rows)
+    _lib.call_on(dev, _lib.entry("qd_kv_read_fp8"), *where, k.data_ptr(), v.data_ptr(), b, h, rows)
     return k, v

@@ -145,15 +145,23 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device``'s current stream as the last argument, whatever the
-    current device is (a kernel launches on the current device only)."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+def call_on(device: int, fn, *args) -> None:
+    """Entry ``fn`` (``entry(name)``) with the current stream of GPU ``device`` as its
+    last argument, whatever the current device is (a kernel launches on the current
+    device only)."""
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        check(status, fn.__name__)
+
+
+@lru_cache(maxsize=None)
+def entry(name: str):
+    """A C entry by name, looked up once."""
+    return getattr(lib(), name)
 
 
 class ModelDesc(ctypes.Structure):
@@ -186,5 +194,5 @@ ModelDesc._fields_ = [
     ("batch_tiled_weights", c_int),
 ]
 
-__all__ = ["lib", "check", "ptr", "stream", "call", "call_on", "QD_F16", "QD_F32", "ModelDesc", "LayerDesc", "EXPORTED",
+__all__ = ["lib", "check", "ptr", "stream", "call", "call_on", "entry", "QD_F16", "QD_F32", "ModelDesc", "LayerDesc", "EXPORTED",
            "LIB_PATH", "c_int64"]

@@ -64,7 +64,7 @@ def test_cpu_tensors_are_refused():
 def test_cache_arguments_are_checked():
     import cuda_decode_small_ops as S
 
-    cpu = torch.device("cpu")
+    cpu = -1   # get_device() of a CPU tensor
     c = S.new_kv_cache_fp8(2, 3, 128, "cpu")
     assert S._kv_fp8_args("t", c, cpu)[:3] == (2, 3, 128)
     assert S._kv_fp8_args("t", [t[1:, ::2] for t in c], cpu)[:3] == (1, 2, 128)
@@ -161,7 +161,7 @@ def test_c_attention_refuses(lib):
         _refused(lib, call(scale=scale), -1, b"scale")
     _refused(lib, call(window=-1), -1, b"window")
     _refused(lib, call(sinks=-1), -1, b"window")
-    for over in (dict(hq=5), dict(sq=-1), dict(sq=1 << 20, hq=4), dict(b=40000)):
+    for over in (dict(hq=5), dict(sq=-1), dict(sq=1 << 22, hq=4), dict(sq=20000, b=32767), dict(b=40000)):
         assert call(**over) == -2, over
     assert call(q=None, sq=0) == 0
     need = lib.qd_attention_fp8_workspace_bytes(1, 1, 16, 8, 32768, 0, 0)
