@@ -292,7 +292,7 @@ int qd_add_rmsnorm_fp8(const void* residual, long ld_residual, const void* x, lo
 /* y[M][N] = x[M][K] W[N][K]^T of 8-bit operands: x_scale [M][ceil(K / 128)],
  * w_scale [ceil(N / 128)][ceil(K / 128)], y in y_dtype.  K a multiple of 16,
  * at most 2^23; M <= 2^20, N <= 2^24; x, w and y 16-byte aligned; products of two
- * scales within fp32's range.  Sums are fp32; of fp16 results for more than 64 rows
+ * scales within fp32's range.  Sums are fp32; of fp16 results for more than 16 rows
  * those of each 8 products at neighbouring k (8 j .. 8 j + 7) keep what is above
  * 2^-13 of the largest of them. */
 int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const void* w_scale, void* y, int y_dtype,

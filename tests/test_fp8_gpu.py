@@ -151,16 +151,18 @@ def _operands(g, m, n, k, cuda):
 def _product_bound(xd, wd, out, dtype):
     """fp32 sums of exact products: K additions, each within 2^-23 of the running
     |sum| <= sum |x w| (to nearest 2^-24; a matrix unit may truncate); then the result's
-    type.  fp16 results of more than 64 rows: of each 8 neighbouring products up to 7
+    type.  fp16 results of more than 16 rows: of each 8 neighbouring products up to 7
     lose what is below 2^-13 of the largest, so at most 7 * 2^-13 of sum |x w|."""
     k, half = xd.shape[1], dtype == torch.float16
-    part = k * 2.0 ** -23 + (7 * 2.0 ** -13 if half and xd.shape[0] > 64 else 0.0)
+    part = k * 2.0 ** -23 + (7 * 2.0 ** -13 if half and xd.shape[0] > 16 else 0.0)
     return part * (xd.abs() @ wd.abs().T) + (2.0 ** -11 * out.abs() + 2.0 ** -25 if half else 2.0 ** -24 * out.abs())
 
 
 SHAPES = [(1, 16, 16), (1, 4096, 2048), (3, 100, 144), (8, 1000, 2048), (16, 129, 6144), (17, 130, 2048), (33, 2048, 400),
           (64, 257, 1040), (65, 300, 2048), (128, 128, 128), (200, 1111, 272), (257, 600, 2048), (300, 128, 6144),
-          (513, 2048, 1008), (1029, 4096, 2048)]
+          (513, 2048, 1008), (1029, 4096, 2048), (5, 60000, 2048), (16, 33000, 1152), (2000, 1500, 1024), (1300, 12288, 576),
+          (2111, 8200, 2048), (700, 1004, 7424), (130, 12288, 144), (770, 500, 144), (1029, 6000, 7296), (1029, 1004, 1152),
+          (1029, 500, 144), (500, 8200, 576), (1029, 8200, 1152), (1029, 8199, 576), (16, 33001, 1040)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
