@@ -91,6 +91,7 @@ int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const
              "need M >= 0, N >= 1 and K a positive multiple of 16 (M=%d N=%d K=%d)", M, N, K);
   QD_REQUIRE(N <= (1 << 24) && M <= (1 << 20) && K <= (1 << 23), QD_ERR_SHAPE,
              "need M <= 2^20, N <= 2^24 and K <= 2^23 (M=%d N=%d K=%d)", M, N, K);
+  QD_REQUIRE((long)M * N <= (1L << 37), QD_ERR_SHAPE, "more than 2^37 results (M=%d N=%d)", M, N);
   if (M == 0) return QD_OK;
   QD_REQUIRE(x && x_scale && w && w_scale && y, QD_ERR_ARG, "null pointer");
   QD_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(y, 16), QD_ERR_ARG, "x, w and y must be 16-byte aligned");

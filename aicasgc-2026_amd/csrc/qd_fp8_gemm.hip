@@ -280,7 +280,8 @@ __device__ __forceinline__ int tile_of_block() {
 // waves.  16-byte chunk c of row r sits at c ^ (r % 8); the permutation is applied to
 // the source address, since the load's LDS side is contiguous.
 //
-// Scales come with their stage, as the aligned words that hold them: each wave loads
+// Scales come with their stage, as the aligned words that hold them (up to 3 bytes of a
+// word are a neighbour's; a word never leaves its scale's allocation): each wave loads
 // one word per lane, lane l < BM / waves the one of its l-th row of x, the others W's.
 //
 // TAIL: the last block is partial (K is a multiple of 16); a chunk past K repeats

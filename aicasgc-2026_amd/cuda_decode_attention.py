@@ -252,7 +252,7 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
         raise RuntimeError(f"{name}: window and sinks must not be negative")
     cp = _positions(name, cache_position, b, dev)
     qi = _strided_heads(q, 8)
-    out = q.new_empty((b, sq, hq, 128))
+    out = torch.empty_strided((b, sq, hq, 128), (sq * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
     need = _fp8_ws_bytes(b, sq, hq, h, t, window, sinks)
     ws = None
     if need:

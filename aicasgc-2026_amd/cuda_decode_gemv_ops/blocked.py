@@ -36,7 +36,7 @@ def block_matmul_fp8(x, x_scale, weight, weight_scale, out_dtype: torch.dtype = 
     if code is None:
         raise RuntimeError(f"{name}: out_dtype must be float16 or float32")
     xi, xs, w, ws = _aligned(x), x_scale.contiguous(), _aligned(weight), weight_scale.contiguous()
-    y = x.new_empty((*lead, n), dtype=out_dtype)
+    y = torch.empty((*lead, n), dtype=out_dtype, device=x.device)
     _lib.call_on(dev, _lib.entry("qd_block_matmul_fp8"), xi.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
                  y.data_ptr(), code, x.numel() // k, n, k)
     return y

@@ -170,6 +170,7 @@ def add(a, b):
 # ---------------------------------------------------------------- 8-bit operators
 
 _F8, _E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_EMPTY_LIKE = torch.empty_like
 FP8_COLS = 128       # columns (and, of a weight, rows) per scale
 KV_FP8_BLOCK = 64    # cache rows per scale
 
@@ -186,10 +187,10 @@ def _half_gpu(name: str, *ts) -> int:
 def _as_rows(t: torch.Tensor):
     """``t`` as rows of its last dimension: (tensor to keep, row stride).  A view
     whose rows follow one another at one stride is used in place."""
-    if t.ndim == 2 and t.stride(1) == 1:
-        return t, t.stride(0)
     if t.is_contiguous():
         return t, t.shape[-1]
+    if t.ndim == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
     if t.ndim > 2 and t.stride(-1) == 1:
         step, rows = t.shape[-1], 1
         for size, stride in zip(t.shape[-2::-1], t.stride()[-2::-1]):
@@ -210,8 +211,14 @@ def _quantized_like(name: str, x: torch.Tensor):
     cols = shape[-1] if shape else 0
     if cols < 1:
         raise RuntimeError(f"{name}: rows must have at least one column")
-    blocks = (cols + FP8_COLS - 1) // FP8_COLS
-    return (x.new_empty(shape, dtype=_F8), x.new_empty((*shape[:-1], blocks), dtype=_E8), x.numel() // cols, cols)
+    blocks, rows = (cols + FP8_COLS - 1) // FP8_COLS, x.numel() // cols
+    # (of the ways to get an empty tensor the two quickest; a decode call's time is its host side's)
+    q = _EMPTY_LIKE(x, dtype=_F8) if x.is_contiguous() else x.new_empty(shape, dtype=_F8)
+    if len(shape) == 2:
+        scale = torch.empty_strided((rows, blocks), (blocks, 1), dtype=_E8, device=x.device)
+    else:
+        scale = x.new_empty((*shape[:-1], blocks), dtype=_E8)
+    return q, scale, rows, cols
 
 
 def quantize_fp8(x, block_rows: int = 1):
@@ -254,7 +261,7 @@ def _norm_fp8(name, dev, residual, x, weight, eps):
     ri, ldr, total, r_ptr, t_ptr = None, 0, None, None, None
     if residual is not None:
         ri, ldr = _as_rows(residual)
-        total = x.new_empty(x.shape)
+        total = _EMPTY_LIKE(x, memory_format=torch.contiguous_format)
         r_ptr, t_ptr = ri.data_ptr(), total.data_ptr()
     _lib.call_on(dev, _lib.entry("qd_add_rmsnorm_fp8"), r_ptr, ldr, xi.data_ptr(), ld, wc.data_ptr(), t_ptr, q.data_ptr(),
                  scale.data_ptr(), rows, cols, eps)
@@ -279,7 +286,8 @@ def rms_norm_fp8(x, weight, eps: float):
 class KVCacheFP8(NamedTuple):
     """The 8-bit KV cache of one layer: rows in blocks of 64 tokens, one scale per
     (sequence, kv head, block) for K and one for V.  V is transposed inside its
-    block.  Views of some sequences or heads are caches too."""
+    block.  Views of some sequences or heads are caches too (one sequence expanded
+    to several can be read, not written)."""
 
     k: torch.Tensor          # e4m3 [B, Hkv, T, 128], T a multiple of 64
     v: torch.Tensor          # e4m3 [B, Hkv, T / 64, 128, 64]
@@ -293,12 +301,13 @@ def new_kv_cache_fp8(batch: int, kv_heads: int, capacity: int, device="cuda") ->
         raise RuntimeError("new_kv_cache_fp8: batch, kv_heads and capacity must be positive")
     nb = (capacity + KV_FP8_BLOCK - 1) // KV_FP8_BLOCK
 
-    def zeros(dtype, *shape):
-        return torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
+    def full(byte, dtype, *shape):
+        return torch.full(shape, byte, dtype=torch.uint8, device=device).view(dtype)
 
-    return KVCacheFP8(zeros(_F8, batch, kv_heads, nb * KV_FP8_BLOCK, 128),
-                      zeros(_F8, batch, kv_heads, nb, 128, KV_FP8_BLOCK),
-                      zeros(_E8, batch, kv_heads, nb), zeros(_E8, batch, kv_heads, nb))
+    # values 0, scales the smallest that a cache has, 2^-32
+    return KVCacheFP8(full(0, _F8, batch, kv_heads, nb * KV_FP8_BLOCK, 128),
+                      full(0, _F8, batch, kv_heads, nb, 128, KV_FP8_BLOCK),
+                      full(127 - 32, _E8, batch, kv_heads, nb), full(127 - 32, _E8, batch, kv_heads, nb))
 
 
 def _kv_fp8_args(name: str, cache, dev: int):
@@ -358,6 +367,8 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
         raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128]")
     bs, s, hq, d = q.shape
     b, h, t, where = _kv_fp8_args(name, cache, dev)
+    if (b > 1 and where[4] == 0) or (h > 1 and where[5] == 0):
+        raise RuntimeError(f"{name}: sequences (or heads) that share their rows cannot be written")
     if d != 128 or k.shape != (bs, s, h, 128) or v.shape != (bs, s, h, 128) or bs != b:
         raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128], with the cache's B and Hkv")
     if hq % h or not h <= hq <= 64 * h:
@@ -369,7 +380,7 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
     cp = _positions(name, cache_position, b, dev)
     qi, ki, vi = _strided_heads(q, 4), _strided_heads(k, 4), _strided_heads(v, 4)
     qw, kw, cs, sn = q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous()
-    out = q.new_empty((b, s, hq, 128))
+    out = torch.empty_strided((b, s, hq, 128), (s * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
     _lib.call_on(dev, _lib.entry("qd_q_rope_kv_update_fp8"), qi.data_ptr(), *qi.stride()[:3], ki.data_ptr(), *ki.stride()[:3],
                  vi.data_ptr(), *vi.stride()[:3], qw.data_ptr(), kw.data_ptr(), eps, cs.data_ptr(), sn.data_ptr(),
                  out.data_ptr(), *where, cp.data_ptr(), b, s, hq, h)

@@ -291,7 +291,7 @@ int qd_add_rmsnorm_fp8(const void* residual, long ld_residual, const void* x, lo
 
 /* y[M][N] = x[M][K] W[N][K]^T of 8-bit operands: x_scale [M][ceil(K / 128)],
  * w_scale [ceil(N / 128)][ceil(K / 128)], y in y_dtype.  K a multiple of 16,
- * at most 2^23; M <= 2^20, N <= 2^24; x, w and y 16-byte aligned; products of two
+ * at most 2^23; M <= 2^20, N <= 2^24, M N <= 2^37; x, w and y 16-byte aligned; products of two
  * scales within fp32's range.  Sums are fp32; of fp16 results for more than 16 rows
  * those of each 8 products at neighbouring k (8 j .. 8 j + 7) keep what is above
  * 2^-13 of the largest of them. */
@@ -302,7 +302,8 @@ int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const
  * k_cache [T][128] per head, v_cache [T / 64][128][64] per head (each 64-row block
  * transposed), batch and head strides stride_b and stride_h in bytes for both;
  * k_scale and v_scale [T / 64] per head, strides scale_stride_b and
- * scale_stride_h.  Heads are contiguous and 16-byte aligned.
+ * scale_stride_h.  Heads are contiguous and 16-byte aligned; a scale is at least
+ * 2^-32 (byte 95), in blocks that nothing was written to as well.
  *
  * qd_q_rope_kv_update_fp8: RMSNorm (head_dim 128) + rotate-half RoPE of q and k for
  * S new tokens of each sequence, cos / sin fp16 [B][S][128]; q_out fp16

@@ -517,6 +517,52 @@ def test_nan_in_rows_that_are_not_seen(cuda, sq, window):
     assert int(out.isnan().sum()) == 2   # the two q heads of kv head 1, one dim, the last token
 
 
+@pytest.mark.parametrize("sq", [1, 60])
+def test_nan_in_a_key_or_query_that_is_seen(cuda, sq):
+    """A visible K row or a query with a NaN makes its own rows NaN, all of them, and
+    no others."""
+    import cuda_decode_small_ops as S
+
+    q, cache = _attend_inputs(S, cuda, 1, 4, 2, sq, 256, seed=5)
+    last = 200
+    cache.k.view(torch.uint8)[0, 1, last, 9] = 0x7F       # seen by the last token only
+    q[0, 1, 0, 3] = float("nan")                          # head 1, first token
+    q[0, 0, 0, 5] = float("inf")
+    out = _attend_check(q, cache, [last + 1 - sq], what=f"NaN in K, Sq={sq}")
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, -1, 2:], bad[0, 0, :2] = True, True
+    assert torch.equal(out.isnan(), bad)
+
+
+def test_rows_of_a_fresh_cache_count_as_zeros(cuda):
+    """Rows that were never written are zeros with a weight like any other."""
+    import cuda_decode_small_ops as S
+
+    for sq in (1, 70):
+        fresh = S.new_kv_cache_fp8(2, 2, 300, cuda)
+        t = _new_tokens(_gen(3), 2, 80, 4, 2)
+        _update(S, t, fresh, [0, 128], cuda)
+        q = _randn(_gen(6), 2, sq, 4, 128).to(cuda).transpose(1, 2)
+        _attend_check(q, fresh, [300 - sq, 299 - sq], what=f"fresh rows Sq={sq}")
+
+
+def test_one_prefix_shared_by_a_batch(cuda):
+    """One sequence's cache expanded to several is read; writing through it is refused."""
+    import cuda_decode_attention as A
+    import cuda_decode_small_ops as S
+
+    q, cache = _attend_inputs(S, cuda, 4, 4, 2, 2, 256, seed=8)
+    shared = S.KVCacheFP8(*(t[:1].expand(4, *t.shape[1:]) for t in cache))
+    pos = torch.tensor([100, 254, 3, 77], device=cuda)
+    out = A.attn_fp8_kv_cache(q, shared, SCALE, pos)
+    for b in range(4):
+        one = A.attn_fp8_kv_cache(q[b:b + 1], S.KVCacheFP8(*(t[:1] for t in cache)), SCALE, pos[b:b + 1])
+        assert torch.equal(out[b:b + 1], one)
+    t = _new_tokens(_gen(2), 4, 1, 4, 2)
+    with pytest.raises(RuntimeError, match="share"):
+        _update(S, t, shared, [0, 1, 2, 3], cuda)
+
+
 def test_one_visible_row_is_returned(cuda):
     import cuda_decode_attention as A
     import cuda_decode_small_ops as S
