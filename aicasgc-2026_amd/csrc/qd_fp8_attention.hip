@@ -37,23 +37,27 @@ constexpr float kProbExp = 9.f;
 constexpr float kMaxLag = 6.f;   // 2^(9 + 6) is within fp16
 constexpr float kLowest = -3.402823466e38f;   // running maximum of a row that has seen nothing
 
-// The cache tiles that query tokens [t0, t1] of a sequence see: the sink tiles
-// [0, ns) and the tiles [first, first + n - ns).
+// The cache tiles that query tokens at [p_min, p_max] of a sequence see: the sink tiles
+// [0, ns) and the tiles [first, first + n - ns); of those, [full0, full1) and [0, sink_full)
+// are visible to every one of them as a whole.
 struct TileRange {
-  long first;
-  int ns, n;
-  __device__ __forceinline__ long tile(int v) const { return v < ns ? v : first + (v - ns); }
+  int first, ns, n, full0, full1, sink_full;
+  __device__ __forceinline__ int tile(int v) const { return v < ns ? v : first + (v - ns); }
+  __device__ __forceinline__ bool masked(int t) const { return !((t >= full0 && t < full1) || t < sink_full); }
 };
 __device__ __forceinline__ TileRange visible_tiles(long p_min, long p_max, const AttnFp8Args& a) {
-  TileRange r{0, 0, 0};
+  TileRange r{0, 0, 0, 0, 0, 0};
   const long hi = min(p_max + 1, (long)a.c.T);
   if (hi <= 0) return r;
-  const long end = (hi + kKvBlock - 1) >> 6;
+  const int end = (int)((hi + kKvBlock - 1) >> 6);
+  r.full1 = (int)(max(min(p_min + 1, (long)a.c.T), 0L) >> 6);
   if (a.window > 0) {
-    r.first = min(max(p_min - a.window + 1, 0L) >> 6, end);
-    r.ns = (int)min((min((long)a.sinks, hi) + kKvBlock - 1) >> 6, r.first);
+    r.first = (int)min(max(p_min - a.window + 1, 0L) >> 6, (long)end);
+    r.ns = min((int)((min((long)a.sinks, hi) + kKvBlock - 1) >> 6), r.first);
+    r.full0 = (int)min((max(p_max - a.window + 1, 0L) + kKvBlock - 1) >> 6, (long)end);
+    r.sink_full = min(a.sinks >> 6, r.full1);
   }
-  r.n = r.ns + (int)(end - r.first);
+  r.n = r.ns + end - r.first;
   return r;
 }
 
@@ -126,13 +130,6 @@ __device__ __forceinline__ void scores(f32x4 (&s)[QT][4], Q q, F load) {
       }
     }
   }
-}
-
-// Whether some token of the tile at `base` is hidden from some row.
-template <int QT>
-__device__ __forceinline__ bool is_masked(const Rows<QT>& w, const long base, const AttnFp8Args& a) {
-  return !(base + kKvBlock - 1 <= w.p_min &&
-           (a.window == 0 || base > w.p_max - a.window || base + kKvBlock <= a.sinks));
 }
 
 // Bit 4 n + j: this lane's token (n, j) of the tile at `base` is visible to its row i.
@@ -242,8 +239,8 @@ __device__ __forceinline__ void mark_nan(Rows<QT>& w, const TileRange& tr, int v
                                          const AttnFp8Args& a, const int g) {
 #pragma unroll 1
   for (; v < v1; v += step) {
+    if (!tr.masked(tr.tile(v))) continue;
     const long t = tr.tile(v), base = t * kKvBlock;
-    if (!is_masked(w, base, a)) continue;
     unsigned any = 0u;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
@@ -412,7 +409,7 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
     __builtin_amdgcn_sched_barrier(0);
     h8v p[1][2];
     const long base = tr.tile(v) * kKvBlock;
-    const bool masked = is_masked(rows, base, a);
+    const bool masked = tr.masked(tr.tile(v));
     mask_and_max<1>(rows, s[x], fac[x], vs_byte - 127, masked, base, a, g);
     if (masked) {
 #pragma unroll
@@ -563,7 +560,7 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
     char* st = attention_stage<x>() + stream * 2 * kTileBytes;
     auto vrow = [&](int d) { return reinterpret_cast<u32x4*>(st + vo + 16 * d * kKvBlock); };
     const long base = tr.tile(v) * kKvBlock;
-    const bool masked = is_masked(rows, base, a);
+    const bool masked = tr.masked(tr.tile(v));
     mask_and_max<2>(rows, s[x], fac, ev, masked, base, a, g);
     if (masked) {   // (in place: the wave of the other rows does the same to the same tile)
 #pragma unroll
