@@ -115,9 +115,9 @@ int qd_q_rope_kv_update_fp8(const void* q, long q_sb, long q_ss, long q_sh, cons
              "Hq must be 1 to 64 times Hkv (Hq=%d Hkv=%d)", Hq, Hkv);
   if (B == 0 || S_ == 0) return QD_OK;
   QD_REQUIRE(q && k && v && q_weight && k_weight && cos && sin && q_out && cache_position, QD_ERR_ARG, "null pointer");
-  QD_REQUIRE(aligned(q, 8) && aligned(k, 8) && aligned(v, 8) && aligned(q_out, 8) && aligned(cos, 2) && aligned(sin, 2) &&
-                 aligned(q_weight, 2) && aligned(k_weight, 2) && aligned(cache_position, 8),
-             QD_ERR_ARG, "q, k, v and q_out must be 8-byte aligned");
+  QD_REQUIRE(aligned(q, 8) && aligned(k, 8) && aligned(v, 8) && aligned(q_out, 8) && aligned(cos, 8) && aligned(sin, 8) &&
+                 aligned(q_weight, 8) && aligned(k_weight, 8) && aligned(cache_position, 8),
+             QD_ERR_ARG, "every operand must be 8-byte aligned");
   QD_REQUIRE(((q_sb | q_ss | q_sh | k_sb | k_ss | k_sh | v_sb | v_ss | v_sh) & 3) == 0, QD_ERR_ARG,
              "q, k and v strides must be multiples of 4 elements");
   a.q = (const u16*)q; a.q_sb = q_sb; a.q_ss = q_ss; a.q_sh = q_sh;

@@ -349,6 +349,13 @@ def _strided_heads(t: torch.Tensor, multiple: int) -> torch.Tensor:
     return t if not t.data_ptr() % (2 * multiple) else t.clone()
 
 
+def _aligned8(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it, contiguous at an 8-byte aligned address."""
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if not t.data_ptr() % 8 else t.clone()
+
+
 def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, cos, sin, cache: KVCacheFP8,
                                      cache_position):
     """q/k per-head RMSNorm + RoPE of S new tokens of each sequence, their K_rot and V
@@ -379,7 +386,7 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
         raise RuntimeError(f"{name}: cos/sin must be [B, S, 128]")
     cp = _positions(name, cache_position, b, dev)
     qi, ki, vi = _strided_heads(q, 4), _strided_heads(k, 4), _strided_heads(v, 4)
-    qw, kw, cs, sn = q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous()
+    qw, kw, cs, sn = _aligned8(q_weight), _aligned8(k_weight), _aligned8(cos), _aligned8(sin)
     out = torch.empty_strided((b, s, hq, 128), (s * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
     _lib.call_on(dev, _lib.entry("qd_q_rope_kv_update_fp8"), qi.data_ptr(), *qi.stride()[:3], ki.data_ptr(), *ki.stride()[:3],
                  vi.data_ptr(), *vi.stride()[:3], qw.data_ptr(), kw.data_ptr(), eps, cs.data_ptr(), sn.data_ptr(),

@@ -123,8 +123,8 @@ def test_c_matmul_refuses(lib):
 
 
 def test_c_cache_entries_refuse(lib):
-    def update(q=A16, kc=A16, sb=8192, T=64, pos=A16, b=1, s=1, hq=4, hkv=2, qs=512):
-        return lib.qd_q_rope_kv_update_fp8(q, qs, qs, 128, A16, 256, 256, 128, A16, 256, 256, 128, A16, A16, 1e-6, A16, A16,
+    def update(q=A16, kc=A16, cos=A16, sb=8192, T=64, pos=A16, b=1, s=1, hq=4, hkv=2, qs=512):
+        return lib.qd_q_rope_kv_update_fp8(q, qs, qs, 128, A16, 256, 256, 128, A16, 256, 256, 128, A16, A16, 1e-6, cos, A16,
                                            A16, kc, A16, A16, A16, sb, 8192, 1, 1, T, pos, b, s, hq, hkv, None)
 
     _refused(lib, update(T=100), -2, b"multiple of 64")
@@ -133,6 +133,7 @@ def test_c_cache_entries_refuse(lib):
     _refused(lib, update(sb=8200), -1, b"aligned")
     _refused(lib, update(q=None), -1, b"null")
     _refused(lib, update(q=A16 + 4), -1, b"aligned")
+    _refused(lib, update(cos=A16 + 2), -1, b"aligned")
     _refused(lib, update(qs=510), -1, b"strides")
     _refused(lib, update(pos=A16 + 4), -1, b"aligned")
     for over in (dict(hq=3), dict(hq=130), dict(hkv=0), dict(s=-1), dict(b=40000)):

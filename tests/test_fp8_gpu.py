@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 
 EPS = 1e-6
 FP32 = 2.0 ** -18   # relative part of the fp32 arithmetic before a rounding to e4m3: RMSNorm's sum of squares
-                    # is at most 50 additions deep (8 per 2048 columns, 8 lane and wave steps), exp 2 ulp
+                    # is at most 50 additions deep (8 per 2048 columns, 8 lane and wave steps), SiLU 4 steps
 
 
 def _bytes(t):
@@ -122,6 +122,31 @@ def test_silu_mul_rows_of_a_fused_product(cuda, rows, cols):
     q, s = S.fused_silu_mul_fp8(gate, up)
     t = gu.double()
     _check_quantized(q, s, t[:, :cols] / (1 + torch.exp(-t[:, :cols])) * t[:, cols:], what=f"silu {rows}x{cols}")
+
+
+def test_silu_keeps_its_precision_far_out(cuda):
+    """Gates of one size per block, from -80 to 80: e^-v has |v| times the rounding of its
+    exponent unless that is made up for."""
+    import cuda_decode_small_ops as S
+
+    g = _gen(4)
+    gate = torch.tensor([-80.0, -60, -30, -5, -1e-3, 0, 1e-3, 5, 30, 80]).half()[:, None] + _randn(g, 10, 128, std=0.05)
+    up = _randn(g, 10, 128)
+    q, s = S.fused_silu_mul_fp8(gate.to(cuda), up.to(cuda))
+    t = gate.double()
+    _check_quantized(q, s, t / (1 + torch.exp(-t)) * up.double(), what="silu far out")
+
+
+def test_silu_of_every_finite_gate(cuda):
+    """All 63488 finite fp16 gates in order, 128 neighbours to a block."""
+    import cuda_decode_small_ops as S
+
+    g = torch.arange(0x7C00, dtype=torch.int16).view(torch.float16)
+    g = torch.cat([-g.flip(0), g]).view(-1, 128)
+    q, s = S.fused_silu_mul_fp8(g.to(cuda), torch.ones_like(g).to(cuda))
+    assert not torch.isnan(q.float()).any()
+    t = g.double()
+    _check_quantized(q, s, t / (1 + torch.exp(-t)), what="silu of every gate")
 
 
 def test_rows_at_odd_strides_and_ranks(cuda):
@@ -385,6 +410,13 @@ def test_cache_update_takes_strided_inputs(cuda):
                                             EPS, t["cos"].to(cuda), t["sin"].to(cuda), b, cp)
     assert torch.equal(q1, q2)
     for x, y in zip(a, b):
+        assert torch.equal(_bytes(x), _bytes(y))
+    # operands at odd addresses are copied
+    odd = {n: torch.empty(v.numel() + 1, dtype=torch.float16, device=cuda)[1:].view(v.shape).copy_(v) for n, v in t.items()}
+    c = _filled(S, 2, 2, 128, cuda)
+    q3 = S.fused_q_rope_kv_cache_update_fp8(odd["q"], odd["k"], odd["v"], odd["qw"], odd["kw"], EPS, odd["cos"], odd["sin"], c, cp)
+    assert torch.equal(q1, q3)
+    for x, y in zip(a, c):
         assert torch.equal(_bytes(x), _bytes(y))
 
 
