@@ -238,7 +238,7 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
 
     ``workspace`` keeps the kernel's scratch memory between calls (it holds nothing
     from one call to the next, so it needs no clearing, but two calls in flight at
-    once must not share it).  Unlike the other entry points, inputs outside what the
+    once must not share it; a graph captured with it needs the dict kept alive).  Unlike the other entry points, inputs outside what the
     kernel supports raise RuntimeError: there is no other path over this cache."""
     name = "attn_fp8_kv_cache"
     dev = _half_gpu(name, q)
@@ -248,19 +248,22 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
     bq, hq, sq, d = q.shape
     if d != 128 or bq != b or hq < h or hq % h:
         raise RuntimeError(f"{name}: q must be [B, Hq, Sq, 128] with the cache's batch and a multiple of its kv heads")
-    if window < 0 or sinks < 0:
-        raise RuntimeError(f"{name}: window and sinks must not be negative")
+    if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
+        raise RuntimeError(f"{name}: window and sinks must lie in [0, 2^31)")
     cp = _positions(name, cache_position, b, dev)
     qi = _strided_heads(q, 8)
     out = torch.empty_strided((b, sq, hq, 128), (sq * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
     need = _fp8_ws_bytes(b, sq, hq, h, t, window, sinks)
     ws = None
     if need:
-        ws = workspace.get(_FP8_WS_KEY) if workspace is not None else None
-        if ws is None or ws.numel() < need or ws.get_device() != dev:
+        key = (_FP8_WS_KEY, dev)
+        ws = workspace.get(key) if workspace is not None else None
+        if ws is None or ws.numel() < need:
+            if ws is not None:   # stays: a captured graph may go on writing to it
+                workspace.setdefault(key + ("outgrown",), []).append(ws)
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             if workspace is not None:
-                workspace[_FP8_WS_KEY] = ws
+                workspace[key] = ws
     _lib.call_on(dev, _lib.entry("qd_attention_fp8"), qi.data_ptr(), *qi.stride()[:3], *where, cp.data_ptr(), scaling, window,
                  sinks, out.data_ptr(), b, sq, hq, h, None if ws is None else ws.data_ptr(), need)
     return out

@@ -17,7 +17,7 @@ def block_matmul_fp8(x, x_scale, weight, weight_scale, out_dtype: torch.dtype = 
     x [..., K] with x_scale [..., ceil(K / 128)] (``cuda_decode_small_ops.quantize_fp8``
     and the ``fused_*_fp8`` entry points), weight [N, K] with weight_scale
     [ceil(N / 128), ceil(K / 128)] (``quantize_fp8(w, block_rows=128)``); K a
-    multiple of 16.  From one row (a decode token) to thousands (a prompt)."""
+    multiple of 16.  From one row (a decode token) to 2^20 (thousands: a prompt)."""
     name = "block_matmul_fp8"
     dev = x.get_device()
     if (x.dtype is not _F8 or weight.dtype is not _F8 or x_scale.dtype is not _E8 or weight_scale.dtype is not _E8
@@ -30,8 +30,8 @@ def block_matmul_fp8(x, x_scale, weight, weight_scale, out_dtype: torch.dtype = 
     kb = (k + 127) // 128
     if x.shape[-1] != k or x_scale.shape != (*lead, kb) or weight_scale.shape != ((n + 127) // 128, kb):
         raise RuntimeError(f"{name}: need x [..., {k}] with scales [..., {kb}] and weight scales [{(n + 127) // 128}, {kb}]")
-    if n < 1 or k < 16 or k % 16:
-        raise RuntimeError(f"{name}: K must be a positive multiple of 16 and N positive")
+    if n < 1 or k < 16 or k % 16 or x.numel() // k > 1 << 20:
+        raise RuntimeError(f"{name}: K must be a positive multiple of 16, N positive and x of at most 2^20 rows")
     code = _OUT.get(out_dtype)
     if code is None:
         raise RuntimeError(f"{name}: out_dtype must be float16 or float32")

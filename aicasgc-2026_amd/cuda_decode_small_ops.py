@@ -374,8 +374,8 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
         raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128]")
     bs, s, hq, d = q.shape
     b, h, t, where = _kv_fp8_args(name, cache, dev)
-    if (b > 1 and where[4] == 0) or (h > 1 and where[5] == 0):
-        raise RuntimeError(f"{name}: sequences (or heads) that share their rows cannot be written")
+    if (b > 1 and 0 in where[4:7:2]) or (h > 1 and 0 in where[5:8:2]):
+        raise RuntimeError(f"{name}: sequences (or heads) that share their rows or scales cannot be written")
     if d != 128 or k.shape != (bs, s, h, 128) or v.shape != (bs, s, h, 128) or bs != b:
         raise RuntimeError(f"{name}: q must be [B, S, Hq, 128], k and v [B, S, Hkv, 128], with the cache's B and Hkv")
     if hq % h or not h <= hq <= 64 * h:

@@ -593,6 +593,8 @@ def test_one_prefix_shared_by_a_batch(cuda):
     t = _new_tokens(_gen(2), 4, 1, 4, 2)
     with pytest.raises(RuntimeError, match="share"):
         _update(S, t, shared, [0, 1, 2, 3], cuda)
+    with pytest.raises(RuntimeError, match="share"):   # rows of their own, one set of scales
+        _update(S, t, S.KVCacheFP8(cache.k, cache.v, shared.k_scale, shared.v_scale), [0, 1, 2, 3], cuda)
 
 
 def test_one_visible_row_is_returned(cuda):
@@ -691,6 +693,83 @@ def test_equal_calls_give_equal_bits(cuda):
         assert torch.equal(A.attn_fp8_kv_cache(q, cache, SCALE, pos, workspace=ws), first)
     side.synchronize()
     assert torch.equal(other, first)
+
+
+def test_a_captured_call_keeps_its_workspace(cuda):
+    """A larger call replaces the dict's workspace; what a graph captured with the first
+    one writes to is not handed to anyone else."""
+    import cuda_decode_attention as A
+    import cuda_decode_small_ops as S
+
+    q, cache = _attend_inputs(S, cuda, 2, 16, 8, 3, 8192, seed=5)
+    pos = torch.tensor([8000, 4321], device=cuda)
+    small = [q[:1, :, :1], S.KVCacheFP8(*(t[:1] for t in cache)), SCALE, pos[:1]]
+    ws = {}
+    want = A.attn_fp8_kv_cache(*small, workspace=ws)
+    size = sum(t.numel() for t in ws.values())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = A.attn_fp8_kv_cache(*small, workspace=ws)
+    A.attn_fp8_kv_cache(q, cache, SCALE, pos, workspace=ws)
+    others = [torch.full((size,), 7, dtype=torch.uint8, device=cuda) for _ in range(8)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and all((o == 7).all() for o in others)
+        A.attn_fp8_kv_cache(q, cache, SCALE, pos, workspace=ws)
+
+
+def test_refusals_before_any_launch(cuda):
+    import cuda_decode_attention as A
+    import cuda_decode_gemv as G
+    import cuda_decode_small_ops as S
+
+    def h(*shape):
+        return torch.ones(shape, dtype=torch.float16, device=cuda)
+
+    x, w = h(2, 256), h(256)
+    qx, sx = S.quantize_fp8(x)
+    wq, wsc = S.quantize_fp8(h(130, 256), block_rows=128)
+    cache = S.new_kv_cache_fp8(2, 2, 128, cuda)
+    pos = torch.zeros(2, dtype=torch.int64, device=cuda)
+    q, kv, cs = h(2, 1, 4, 128), h(2, 1, 2, 128), h(2, 1, 128)
+
+    def update(q=q, k=kv, v=kv, qw=h(128), cos=cs, cache=cache, pos=pos):
+        return S.fused_q_rope_kv_cache_update_fp8(q, k, v, qw, h(128), EPS, cos, cs, cache, pos)
+
+    def attend(q=q.transpose(1, 2), cache=cache, scale=SCALE, pos=pos, **more):
+        return A.attn_fp8_kv_cache(q, cache, scale, pos, **more)
+
+    calls = [
+        lambda: S.quantize_fp8(x.float()), lambda: S.quantize_fp8(x.cpu()), lambda: S.quantize_fp8(x, block_rows=64),
+        lambda: S.quantize_fp8(x[None], block_rows=128), lambda: S.quantize_fp8(x[:, :0]),
+        lambda: S.fused_silu_mul_fp8(x, x[:1]), lambda: S.fused_add_rms_norm_fp8(x, x[:1], w, EPS),
+        lambda: S.rms_norm_fp8(x, w[:255], EPS), lambda: S.rms_norm_fp8(x, w.bfloat16(), EPS),
+        lambda: G.block_matmul_fp8(x, sx, wq, wsc), lambda: G.block_matmul_fp8(qx, sx.view(torch.uint8), wq, wsc),
+        lambda: G.block_matmul_fp8(qx, sx[:, :1], wq, wsc), lambda: G.block_matmul_fp8(qx, sx, wq, wsc[:1]),
+        lambda: G.block_matmul_fp8(qx[:, :128], sx[:, :1], wq, wsc), lambda: G.block_matmul_fp8(qx, sx, wq, wsc, torch.bfloat16),
+        lambda: G.block_matmul_fp8(qx[:, :24], sx[:, :1], wq[:, :24], wsc[:, :1]),
+        lambda: G.block_matmul_fp8(qx[:1].expand((1 << 20) + 1, 256), sx[:1].expand((1 << 20) + 1, 2), wq, wsc),
+        lambda: S.new_kv_cache_fp8(0, 2, 64, cuda), lambda: S.new_kv_cache_fp8(1, 2, 0, cuda),
+        lambda: S.read_kv_cache_fp8(cache, 129), lambda: S.read_kv_cache_fp8(cache, -1),
+        lambda: S.read_kv_cache_fp8(cache._replace(v=cache.v.transpose(3, 4)), 1),
+        lambda: S.read_kv_cache_fp8(cache._replace(k=cache.k.view(torch.uint8)), 1),
+        lambda: S.read_kv_cache_fp8(cache._replace(k=cache.k[:, :, :100]), 1),
+        lambda: S.read_kv_cache_fp8(cache._replace(k_scale=cache.k_scale[:, :1]), 1),
+        lambda: S.read_kv_cache_fp8(cache._replace(k=cache.k[:, :, ::2]), 1),
+        lambda: update(q=h(2, 1, 3, 128)), lambda: update(q=h(2, 1, 2 * 65, 128)), lambda: update(k=h(2, 2, 2, 128)),
+        lambda: update(v=kv.cpu()), lambda: update(qw=h(64)), lambda: update(cos=h(1, 1, 128)), lambda: update(pos=pos.int()),
+        lambda: update(pos=pos[:1]), lambda: update(q=q[..., :64]),
+        lambda: attend(q=h(2, 3, 1, 128)), lambda: attend(q=h(1, 4, 1, 128)), lambda: attend(q=q.transpose(1, 2).float()),
+        lambda: attend(window=-1), lambda: attend(sinks=-1), lambda: attend(window=1 << 31), lambda: attend(sinks=(1 << 32) + 1),
+        lambda: attend(scale=0.0), lambda: attend(scale=-1.0), lambda: attend(scale=float("nan")),
+        lambda: attend(scale=float("inf")), lambda: attend(pos=pos.cpu()), lambda: attend(pos=pos[None]),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            call()
+            print(f"call {i} was not refused", flush=True)
 
 
 # ---------------------------------------------------------------- together
