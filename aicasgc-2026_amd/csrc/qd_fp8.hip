@@ -1,6 +1,7 @@
 // 8-bit quantisers for gfx950: activation rows (add + RMSNorm, SiLU * up, plain),
 // weight blocks, and the KV cache written in 8 bits and read back.  All are bound by
-// memory or, for a decode token, by their launch.
+// memory or, for a decode token, by their launch.  Sums and maxima are fp32; the one
+// rounding of a stored value is its own to e4m3 (the scales are powers of two).
 
 #include <math.h>
 
@@ -93,7 +94,9 @@ __device__ __forceinline__ void add_row8(float* v, const float* r) {
 
 // One row per workgroup: v = x (+ residual, also stored as fp16), RMSNorm of the
 // fp32 sum, quantised.  C chunks of 2048 columns stay in registers between the two
-// passes; C = 0 (longer rows) reads them again.
+// passes; C = 0 (longer rows) reads them again.  A row per workgroup: its sum needs one
+// exchange of four waves, and 16 lanes hold a scale's 128 columns.  2048 columns with a
+// residual: 4001 rows 12.2 us (4.7 TB/s; a copy of that size reaches 5.1), one row 2.0.
 template <int C, bool VEC>
 __global__ __launch_bounds__(kRowThreads) void add_rmsnorm_fp8_kernel(const RowQuantArgs a) {
   __shared__ float s_red[kRowThreads / kWave];
@@ -155,7 +158,8 @@ __global__ __launch_bounds__(kRowThreads) void add_rmsnorm_fp8_kernel(const RowQ
   }
 }
 
-// 2048 columns of one row per workgroup: x, or silu(x) * x2.
+// 2048 columns of one row per workgroup: x, or silu(x) * x2.  4001 rows: 2048 columns of x
+// 5.3 us (4.6 TB/s), 6144 of silu(x) * x2 22.5 us (5.5 TB/s); one row of 6144 2.4 us.
 template <bool SILU, bool VEC>
 __global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(const RowQuantArgs a) {
   const long row = blockIdx.x, k = (long)blockIdx.y * kRowSpan + threadIdx.x * 8;
@@ -172,7 +176,8 @@ __global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(const RowQua
   quantize8<VEC>(a, row, k, v);
 }
 
-// One 128 x 128 block of a weight per workgroup.
+// One 128 x 128 block of a weight per workgroup, in registers between its maximum and its
+// rounding.  12288 x 2048: 15.6 us (4.8 TB/s).
 template <bool VEC>
 __global__ __launch_bounds__(kRowThreads) void quantize_blocks_kernel(const RowQuantArgs a) {
   __shared__ float s_red[kRowThreads / kWave];
@@ -288,6 +293,10 @@ __device__ __forceinline__ float block_max4(float m, float* s_red) {
 // larger one; then the earlier rows are read, scaled down and written again (exact
 // but for values that become subnormal).  One workgroup owns the block, so nobody
 // else touches those bytes.  Rows behind the new ones keep their bytes.
+//
+// Bound by memory: 4001 tokens of 16 + 2 * 8 heads 14.1 us (60 MB, 4.2 TB/s).  One token of
+// 8 sequences takes 5.7 us, the chain of dependent loads position, row, scale,
+// earlier rows of the block.
 __global__ __launch_bounds__(256) void kv_update_fp8_kernel(const KvUpdateFp8Args a) {
   __shared__ float s_red[4];
   const int b = (int)blockIdx.z / a.c.Hkv, kvh = (int)blockIdx.z % a.c.Hkv;
@@ -438,7 +447,7 @@ int kv_update_fp8_launch(const KvUpdateFp8Args& a, hipStream_t s) {
 
 // One (block, K or V, head) per workgroup: 8 KB in, 16 KB out.  V's 4 dims x 8
 // slots per thread are transposed 4 x 4 bytes at a time, and a wave stores rows of
-// 256 bytes.
+// 256 bytes.  30001 rows of 8 heads: 29.6 us for 184 MB, 6.2 TB/s.
 __global__ __launch_bounds__(256) void kv_read_fp8_kernel(const KvReadFp8Args a) {
   const int b = (int)blockIdx.z / a.c.Hkv, kvh = (int)blockIdx.z % a.c.Hkv;
   const long base = (long)blockIdx.x * kKvBlock;
