@@ -476,7 +476,9 @@ constexpr int kBigMaxBlocks = 56;   // K blocks whose scales fit the LDS of two 
 // here (2.46).  A step of 64 k takes 0.67 us, 3.2 PFLOP/s over the card; each of the three
 // rounds of tiles adds some 9 us for its first loads and its results, which nothing
 // overlaps.  (128 x 256 two per CU 116 us; 256 x 256 with W from memory to
-// registers 137; the fp16 MFMAs 213.)
+// registers 137; the fp16 MFMAs 213.  One workgroup per CU for several tiles, the next one's
+// stages loaded before this one's results are stored: 116, since a wave's loads
+// complete behind its earlier stores, which a new workgroup's do not.)
 template <int BM, int BN, int OCC>
 __global__ __launch_bounds__(256, OCC) void gemm_fp8_big_kernel(const GemmFp8Args a) {
   constexpr int TM = BM / 2, TN = BN / 2, I = TM / 32, J = TN / 32;
