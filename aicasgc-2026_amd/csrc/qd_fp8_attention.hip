@@ -620,6 +620,7 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
 // eighth of the splits and are added through LDS.  3.2 us for 8 splits, 3.9 for 32: two
 // dependent reads and the launch.
 constexpr int kMaxSplits = 64;
+template <int N>   // eights of splits
 __global__ __launch_bounds__(256) void attention_fp8_merge_kernel(const AttnFp8Args a) {
   __shared__ __align__(16) f32x4 s_acc[8][32];
   const int R = a.Sq * a.G;
@@ -627,6 +628,11 @@ __global__ __launch_bounds__(256) void attention_fp8_merge_kernel(const AttnFp8A
   const int r = (int)((long)blockIdx.x % R);
   const long p0 = bh * a.n_split * R + r;
   const int lane = lane_id(), grp = threadIdx.x / 32, d = 4 * (threadIdx.x & 31);
+  // (the partials are loaded before their weights are known: one round trip to memory)
+  f32x4 part[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    part[i] = *reinterpret_cast<const f32x4*>(a.part_o + (p0 + (long)min(8 * i + grp, a.n_split - 1) * R) * kHD + d);
   float m = kLowest, l = 0.f;
   if (lane < a.n_split) {
     m = a.part_ml[2 * (p0 + (long)lane * R)];
@@ -636,11 +642,10 @@ __global__ __launch_bounds__(256) void attention_fp8_merge_kernel(const AttnFp8A
   const float ll = wave_sum(l * wgt);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kMaxSplits / 8; ++i) {
+  for (int i = 0; i < N; ++i) {
     const int s = 8 * i + grp;
-    if (8 * i >= a.n_split) break;
     const float f = __shfl(wgt, s);
-    if (s < a.n_split) acc += *reinterpret_cast<const f32x4*>(a.part_o + (p0 + (long)s * R) * kHD + d) * f;
+    if (s < a.n_split) acc += part[i] * f;
   }
   s_acc[grp][threadIdx.x & 31] = acc;
   __syncthreads();
@@ -672,7 +677,13 @@ int attention_fp8_launch(const AttnFp8Args& a, hipStream_t s) {
                        dim3(512), 0, s, a);
   const int st = qd_host::launch_status("attention_fp8_kernel");
   if (st != QD_OK || a.n_split == 1) return st;
-  hipLaunchKernelGGL(attention_fp8_merge_kernel, dim3((unsigned)(heads * R)), dim3(256), 0, s, a);
+  const dim3 grid((unsigned)(heads * R));
+  if (a.n_split <= 8)
+    hipLaunchKernelGGL(attention_fp8_merge_kernel<1>, grid, dim3(256), 0, s, a);
+  else if (a.n_split <= 32)
+    hipLaunchKernelGGL(attention_fp8_merge_kernel<4>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(attention_fp8_merge_kernel<kMaxSplits / 8>, grid, dim3(256), 0, s, a);
   return qd_host::launch_status("attention_fp8_merge_kernel");
 }
 
