@@ -80,17 +80,17 @@ __device__ __forceinline__ float max_groups(float x) {
 __device__ __forceinline__ unsigned nan_bytes(unsigned v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // A wave's QT x 16 rows (one per column c of each tile, the same in the four
-// lane groups g) and what they have accumulated.
-template <int QT>
+// lane groups g) and what they have accumulated, of 16 ND of the 128 dims.
+template <int QT, int ND = 8>
 struct Rows {
   long p_min, p_max;    // positions of all rows that share this wave's tiles
   int prow[QT];         // each row's, from p_min on (rows past the last repeat it)
-  f32x4 o[QT][8];       // O^T: dims 16 d + 4 g + j
+  f32x4 o[QT][ND];      // O^T: dims 16 d + 4 g + j from the first of its own on
   float m[QT], l[QT];
 };
 
-template <int QT>
-__device__ __forceinline__ void init_rows(Rows<QT>& w, h8v (&q)[QT][4], const AttnFp8Args& a, int b, int kvh, long pos, int r0,
+template <int QT, int ND>
+__device__ __forceinline__ void init_rows(Rows<QT, ND>& w, h8v (&q)[QT][4], const AttnFp8Args& a, int b, int kvh, long pos, int r0,
                                           int R, int c, int g) {
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
@@ -102,7 +102,7 @@ __device__ __forceinline__ void init_rows(Rows<QT>& w, h8v (&q)[QT][4], const At
     w.m[i] = kLowest;
     w.l[i] = 0.f;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) w.o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < ND; ++d) w.o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 }
 
@@ -135,8 +135,8 @@ __device__ __forceinline__ void scores(f32x4 (&s)[QT][4], Q q, F load) {
 }
 
 // Bit 4 n + j: this lane's token (n, j) of the tile at `base` is visible to its row i.
-template <int QT>
-__device__ __forceinline__ unsigned visible_bits(const Rows<QT>& w, const int i, const long base, const AttnFp8Args& a, const int g) {
+template <int QT, int ND>
+__device__ __forceinline__ unsigned visible_bits(const Rows<QT, ND>& w, const int i, const long base, const AttnFp8Args& a, const int g) {
   // bits of the tokens below x of this lane's 16
   auto below = [&](long x) { return 0xffffu >> (16 - min(max((int)min(max(x - base, 0L), (long)kKvBlock) - 16 * g, 0), 16)); };
   const long p = w.p_min + w.prow[i];
@@ -146,8 +146,8 @@ __device__ __forceinline__ unsigned visible_bits(const Rows<QT>& w, const int i,
 }
 
 // Masks a tile's scores and lets the rows' maxima follow them.
-template <int QT>
-__device__ __forceinline__ void mask_and_max(Rows<QT>& w, f32x4 (&s)[QT][4], const float fac, const int ev, const bool masked,
+template <int QT, int ND>
+__device__ __forceinline__ void mask_and_max(Rows<QT, ND>& w, f32x4 (&s)[QT][4], const float fac, const int ev, const bool masked,
                                              const long base, const AttnFp8Args& a, const int g) {
   if (masked) {
 #pragma unroll
@@ -183,14 +183,14 @@ __device__ __forceinline__ void mask_and_max(Rows<QT>& w, f32x4 (&s)[QT][4], con
       w.m[i] = mn;
       w.l[i] *= al;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) w.o[i][d] *= al;
+      for (int d = 0; d < ND; ++d) w.o[i][d] *= al;
     }
   }
 }
 
 // The tile's probabilities in units of the rows' maxima, and their sums.
-template <int QT>
-__device__ __forceinline__ void probabilities(Rows<QT>& w, const f32x4 (&s)[QT][4], const float fac, const int ev,
+template <int QT, int ND>
+__device__ __forceinline__ void probabilities(Rows<QT, ND>& w, const f32x4 (&s)[QT][4], const float fac, const int ev,
                                               h8v (&p)[QT][2]) {
   const float fev = (float)ev, inv = pow2i(-ev);
 #pragma unroll
@@ -210,10 +210,10 @@ __device__ __forceinline__ void probabilities(Rows<QT>& w, const f32x4 (&s)[QT][
 }
 
 // O^T += V^T.P^T; load(d) gives 16 bytes of this lane's V row of dims 16 d.
-template <int QT, typename F>
-__device__ __forceinline__ void accumulate(Rows<QT>& w, const h8v (&p)[QT][2], F load) {
+template <int QT, int ND, typename F>
+__device__ __forceinline__ void accumulate(Rows<QT, ND>& w, const h8v (&p)[QT][2], F load) {
 #pragma unroll
-  for (int d = 0; d < 8; ++d) {
+  for (int d = 0; d < ND; ++d) {
     const u32x4 v = load(d);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -235,9 +235,9 @@ __device__ __forceinline__ u32x4 clean_nan(u32x4 v) {
 }
 
 // tile(v): the v-th of the wave's tiles v, v + step, ... below v1; vp: this lane's V
-// row of dims 0 and token 16 g.
-template <int QT>
-__device__ __forceinline__ void mark_nan(Rows<QT>& w, const TileRange& tr, int v, const int step, const int v1, const uint8_t* vp,
+// row of its first dims and token 16 g.
+template <int QT, int ND>
+__device__ __forceinline__ void mark_nan(Rows<QT, ND>& w, const TileRange& tr, int v, const int step, const int v1, const uint8_t* vp,
                                          const AttnFp8Args& a, const int g) {
 #pragma unroll 1
   for (; v < v1; v += step) {
@@ -245,7 +245,7 @@ __device__ __forceinline__ void mark_nan(Rows<QT>& w, const TileRange& tr, int v
     const long t = tr.tile(v), base = t * kKvBlock;
     unsigned any = 0u;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
+    for (int d = 0; d < ND; ++d) {
       const u32x4 x = ld16(vp + t * kTileBytes + 16 * d * kKvBlock);
       any |= nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w);
     }
@@ -257,7 +257,7 @@ __device__ __forceinline__ void mark_nan(Rows<QT>& w, const TileRange& tr, int v
 #pragma unroll
       for (int e = 0; e < 16; ++e) vis[e / 8][e % 8] = (seen >> e) & 1u ? (_Float16)1.f : (_Float16)0.f;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
+      for (int d = 0; d < ND; ++d) {
         const u32x4 x = ld16(vp + t * kTileBytes + 16 * d * kKvBlock);
         f32x4 cnt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -282,8 +282,8 @@ __device__ __forceinline__ f32x4* row_chunk(char* slot, int r, int x) {
   return reinterpret_cast<f32x4*>(slot + r * (kHD * 4) + 16 * (x ^ (r & 31)));
 }
 // A wave's rows, chunk(r, x) the place of row r's chunk x.
-template <int QT, typename F>
-__device__ __forceinline__ void spill_rows(Rows<QT>& w, F chunk, float (*sml)[2], int c, int g) {
+template <int QT, int ND, typename F>
+__device__ __forceinline__ void spill_rows(Rows<QT, ND>& w, F chunk, float (*sml)[2], int c, int g) {
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const int r = 16 * i + c;
@@ -294,7 +294,7 @@ __device__ __forceinline__ void spill_rows(Rows<QT>& w, F chunk, float (*sml)[2]
       sml[r][1] = w.l[i];
     }
 #pragma unroll
-    for (int d = 0; d < 8; ++d) *chunk(r, 4 * d + g) = w.o[i][d];
+    for (int d = 0; d < ND; ++d) *chunk(r, 4 * d + g) = w.o[i][d];
   }
 }
 
@@ -305,11 +305,12 @@ __device__ __forceinline__ void store_out(const AttnFp8Args& a, int b, int kvh, 
 }
 
 // Joins NS waves' ROWS rows (fixed order), chunk(wave, r, x) the place of a chunk:
-// the result, or a split's partial.
-template <int NS, int ROWS, int NT, typename F>
-__device__ __forceinline__ void join_rows(F chunk, float (*sml)[ROWS][2], const AttnFp8Args& a, int bh, int split, int r0, int R) {
-  for (int n = threadIdx.x; n < ROWS * (kHD / 4); n += NT) {
-    const int rr = n / (kHD / 4), x = n % (kHD / 4), d = 4 * x, r = r0 + rr;
+// the result's dims from d0 on, or a split's partial.
+template <int NS, int ROWS, int NT, int ND, typename F>
+__device__ __forceinline__ void join_rows(F chunk, float (*sml)[ROWS][2], const AttnFp8Args& a, int bh, int split, int r0, int R,
+                                          int d0) {
+  for (int n = threadIdx.x; n < ROWS * 4 * ND; n += NT) {
+    const int rr = n / (4 * ND), x = n % (4 * ND), d = d0 + 4 * x, r = r0 + rr;
     if (r >= R) break;
     float mm = sml[0][rr][0];
 #pragma unroll
@@ -356,23 +357,26 @@ __device__ __forceinline__ int k_token(int c, int n) { return 16 * (c >> 2) + 4 
 // tile ahead are in flight meanwhile.
 //
 // One workgroup per CU (190 registers, eight waves).  Measured, two q rows of each of 8 kv
-// heads: 30001 rows 14.4 us (61 MB, 4.3 TB/s) and 3.9 for the merge, 8 sequences of 2048 to
-// 4096 rows 14.3 and 4.0, 1029 rows 10.5 in one launch, one tile 4.6.  In 1029 rows a wave
-// has two or three tiles, and a CU's 128 KB of tiles more take 3.4 us, so that a short
-// context is bound by the few CUs it fills.  (Four waves and twice the splits: 18.9 us in
-// all for 17.5 at 30001 rows; V two tiles ahead as well, 228 registers: 17.4 for 17.1,
-// and 10.6 for 10.2 at 1029.)
-template <int NW>
+// heads: 30001 rows 14.4 us (61 MB, 4.3 TB/s) and 3 to 4 for the merge, 8 sequences of 2048 to
+// 4096 rows 14.3 and the same, 1029 rows 8.6 in one launch, one tile 4.4.  (Four
+// waves and twice the splits: 18.9 us in all for 17.5 at 30001 rows; V two tiles ahead as
+// well, 228 registers: 17.4 for 17.1.)
+//
+// DS workgroups may share the dims (128 / DS each) and each read all of K: what one CU
+// takes in, some 50 bytes a ns of what memory has to send, falls from 16 KB a tile to
+// 8 + 8 / DS.
+template <int NW, int DS>
 __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8Args a) {
+  constexpr int ND = 8 / DS;
   __shared__ __align__(16) char s_o[NW][16 * kHD * 4];
   __shared__ float s_ml[NW][16][2];
   const int lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;
   const int bh = (int)blockIdx.x, b = bh / a.c.Hkv, kvh = bh % a.c.Hkv;
-  const int split = (int)blockIdx.y, R = a.Sq * a.G;
+  const int split = (int)blockIdx.y, R = a.Sq * a.G, d0 = 16 * ND * (int)blockIdx.z;
   const long pos = a.cache_position[b];
-  Rows<1> rows;
+  Rows<1, ND> rows;
   rows.p_min = pos;
   rows.p_max = pos + a.Sq - 1;
   const TileRange tr = visible_tiles(rows.p_min, rows.p_max, a);
@@ -381,8 +385,8 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
   const long off = b * a.c.stride_b + kvh * a.c.stride_h;
   const long so = b * a.c.scale_stride_b + kvh * a.c.scale_stride_h;
   const uint8_t* kp = a.c.k + off + k_token(c, 0) * kHD + 16 * g;
-  const uint8_t* vp = a.c.v + off + c * kKvBlock + 16 * g;
-  u32x4 kr[4][2], vr[8];
+  const uint8_t* vp = a.c.v + off + (d0 + c) * kKvBlock + 16 * g;
+  u32x4 kr[4][2], vr[ND];
   int ks_byte = 0, vs_byte = 0;   // scales of the tiles in kr and vr
   auto load_k = [&](long t) __attribute__((always_inline)) {
 #pragma unroll
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
   };
   auto load_v = [&](long t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d) vr[d] = ld16(vp + t * kTileBytes + 16 * d * kKvBlock);
+    for (int d = 0; d < ND; ++d) vr[d] = ld16(vp + t * kTileBytes + 16 * d * kKvBlock);
     vs_byte = a.c.v_scale[so + t];
   };
   int v = v0 + w;
@@ -402,7 +406,7 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
     load_v(tr.tile(v));
   }
   h8v q[1][4];
-  init_rows<1>(rows, q, a, b, kvh, pos, 0, R, c, g);
+  init_rows<1, ND>(rows, q, a, b, kvh, pos, 0, R, c, g);
   f32x4 s[2][1][4];
   float fac[2];
   auto next_scores = [&](auto X) __attribute__((always_inline)) {
@@ -420,13 +424,13 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
     h8v p[1][2];
     const long base = tr.tile(v) * kKvBlock;
     const bool masked = tr.masked(tr.tile(v));
-    mask_and_max<1>(rows, s[x], fac[x], vs_byte - 127, masked, base, a, g);
+    mask_and_max<1, ND>(rows, s[x], fac[x], vs_byte - 127, masked, base, a, g);
     if (masked) {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) vr[d] = clean_nan(vr[d]);
+      for (int d = 0; d < ND; ++d) vr[d] = clean_nan(vr[d]);
     }
-    probabilities<1>(rows, s[x], fac[x], vs_byte - 127, p);
-    accumulate<1>(rows, p, [&](int d) { return vr[d]; });
+    probabilities<1, ND>(rows, s[x], fac[x], vs_byte - 127, p);
+    accumulate<1, ND>(rows, p, [&](int d) { return vr[d]; });
     if (v + NW < v1) load_v(tr.tile(v + NW));
   };
   if (v < v1) {
@@ -439,11 +443,11 @@ __global__ __launch_bounds__(kWave * NW) void attention_fp8_kernel(const AttnFp8
     if (v + NW >= v1) break;
     body(std::integral_constant<int, 1>{}, v + NW);
   }
-  mark_nan<1>(rows, tr, v0 + w, NW, v1, vp, a, g);
+  mark_nan<1, ND>(rows, tr, v0 + w, NW, v1, vp, a, g);
   auto chunk = [&](int x, int r, int y) { return row_chunk(s_o[x], r, y); };
-  spill_rows<1>(rows, [&](int r, int y) { return chunk(w, r, y); }, s_ml[w], c, g);
+  spill_rows<1, ND>(rows, [&](int r, int y) { return chunk(w, r, y); }, s_ml[w], c, g);
   __syncthreads();
-  join_rows<NW, 16, kWave * NW>(chunk, s_ml, a, bh, split, 0, R);
+  join_rows<NW, 16, kWave * NW, ND>(chunk, s_ml, a, bh, split, 0, R, d0);
 }
 
 namespace {
@@ -541,7 +545,7 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
   if (v0 < v1) issue(std::integral_constant<int, 1>{}, v0 - kStreams);   // the first tiles' K
   {
     h8v q[2][4];
-    init_rows<2>(rows, q, a, b, kvh, pos, r0 + 32 * half, R, c, g);
+    init_rows<2, 8>(rows, q, a, b, kvh, pos, r0 + 32 * half, R, c, g);
     if (stream < 2)   // one row tile each
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) s_q[half][stream][ks][lane] = stream == 0 ? q[0][ks] : q[1][ks];
@@ -578,7 +582,7 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
     auto vrow = [&](int d) { return reinterpret_cast<u32x4*>(st + vo + 16 * d * kKvBlock); };
     const long base = tr.tile(v) * kKvBlock;
     const bool masked = tr.masked(tr.tile(v));
-    mask_and_max<2>(rows, s[x], fac, ev, masked, base, a, g);
+    mask_and_max<2, 8>(rows, s[x], fac, ev, masked, base, a, g);
     if (masked) {   // (in place: the wave of the other rows does the same to the same tile)
 #pragma unroll
       for (int d = 0; d < 8; ++d) *vrow(d) = clean_nan(*vrow(d));
@@ -587,8 +591,8 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
     // instructions (after the last tile they are of no use)
     h8v p[2][2];
     next_scores(S, other);
-    probabilities<2>(rows, s[x], fac, ev, p);
-    accumulate<2>(rows, p, [&](int d) { return *vrow(d); });
+    probabilities<2, 8>(rows, s[x], fac, ev, p);
+    accumulate<2, 8>(rows, p, [&](int d) { return *vrow(d); });
   };
   wait_barrier();
   if (v0 < v1) {
@@ -602,7 +606,7 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
     step(i0, v);
     if (v + kStreams < v1) step(i1, v + kStreams);
   }
-  if (!idle) mark_nan<2>(rows, tr, v0 + stream, kStreams, v1, a.c.v + off + c * kKvBlock + 16 * g, a, g);
+  if (!idle) mark_nan<2, 8>(rows, tr, v0 + stream, kStreams, v1, a.c.v + off + c * kKvBlock + 16 * g, a, g);
   // join the four streams: the stages are free once every wave is past its last
   // step, each holds the rows of two
   wait_barrier();
@@ -610,15 +614,15 @@ __global__ __launch_bounds__(512, 2) void attention_fp8_many_kernel(const AttnFp
   auto chunk = [&](int x, int r, int y) {
     return row_chunk((x < 2 ? attention_stage<0>() : attention_stage<1>()) + (x & 1) * kManyRows * kHD * 4, r, y);
   };
-  spill_rows<2>(rows, [&](int r, int y) { return chunk(stream, 32 * half + r, y); }, &s_ml[stream][32 * half], c, g);
+  spill_rows<2, 8>(rows, [&](int r, int y) { return chunk(stream, 32 * half + r, y); }, &s_ml[stream][32 * half], c, g);
   __syncthreads();
-  join_rows<kStreams, kManyRows, 512>(chunk, s_ml, a, bh, split, r0, R);
+  join_rows<kStreams, kManyRows, 512, 8>(chunk, s_ml, a, bh, split, r0, R, 0);
 }
 
 // Joins the splits' partials of one row per workgroup, in a fixed order: lane s of a
 // wave holds the weight of split s, eight groups of 32 lanes (4 dims each) sum an
-// eighth of the splits and are added through LDS.  3.2 us for 8 splits, 3.9 for 32: two
-// dependent reads and the launch.
+// eighth of the splits and are added through LDS.  2.8 to 3.8 us: the launch and a
+// read.
 constexpr int kMaxSplits = 64;
 template <int N>   // eights of splits
 __global__ __launch_bounds__(256) void attention_fp8_merge_kernel(const AttnFp8Args a) {
@@ -655,26 +659,37 @@ __global__ __launch_bounds__(256) void attention_fp8_merge_kernel(const AttnFp8A
   store_out(a, (int)(bh / a.c.Hkv), (int)(bh % a.c.Hkv), r, d, acc, ll);
 }
 
+constexpr long kCUs = 256;
+
 int attention_fp8_splits(int B, int Hkv, int Sq, int G, int T, int window, int sinks) {
   long tiles = T / kKvBlock;
   if (window > 0) tiles = min(tiles, ((long)window + Sq + 2 * kKvBlock) / kKvBlock + ((long)sinks + kKvBlock - 1) / kKvBlock);
   const long R = (long)Sq * G;
   const long units = (long)B * Hkv * (R <= 16 ? 1 : (R + kManyRows - 1) / kManyRows);
-  // up to 1536 rows one launch is as quick as two (batch 1, us: 1029 rows 10.4 in one, 12.0
-  // in two; 2048 rows 15.1 / 12.2)
+  // up to 1536 rows one launch is quicker than two (batch 1, us: 1029 rows 9.5 in one, 11.9
+  // in two; 1536 rows 10.5 / 12.5; every 512 rows more add 2 us to one)
   if (tiles <= 24) return 1;
   // one workgroup per CU, a tile or two per wave at least
-  const long n = min(256 / units, (tiles + 7) / 8);
+  const long n = min(kCUs / units, (tiles + 7) / 8);
   return (int)max(1L, min(n, (long)kMaxSplits));
 }
 
 int attention_fp8_launch(const AttnFp8Args& a, hipStream_t s) {
   const long R = (long)a.Sq * a.G, heads = (long)a.c.B * a.c.Hkv;
-  if (R <= 16)
-    hipLaunchKernelGGL((attention_fp8_kernel<8>), dim3((unsigned)heads, (unsigned)a.n_split), dim3(512), 0, s, a);
-  else
+  if (R <= 16) {
+    // the dims of few workgroups are shared while that gives every one a CU of its own (8 kv
+    // heads, us, alone / shared by four: 1029 rows 10.4 / 8.6, 512 7.0 / 6.4, 64 4.6 / 4.4)
+    const long n = heads * a.n_split;
+    if (4 * n <= kCUs)
+      hipLaunchKernelGGL((attention_fp8_kernel<8, 4>), dim3((unsigned)heads, (unsigned)a.n_split, 4), dim3(512), 0, s, a);
+    else if (2 * n <= kCUs)
+      hipLaunchKernelGGL((attention_fp8_kernel<8, 2>), dim3((unsigned)heads, (unsigned)a.n_split, 2), dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL((attention_fp8_kernel<8, 1>), dim3((unsigned)heads, (unsigned)a.n_split), dim3(512), 0, s, a);
+  } else {
     hipLaunchKernelGGL(attention_fp8_many_kernel, dim3((unsigned)(heads * ((R + kManyRows - 1) / kManyRows)), (unsigned)a.n_split),
                        dim3(512), 0, s, a);
+  }
   const int st = qd_host::launch_status("attention_fp8_kernel");
   if (st != QD_OK || a.n_split == 1) return st;
   const dim3 grid((unsigned)(heads * R));

@@ -597,6 +597,25 @@ def test_one_prefix_shared_by_a_batch(cuda):
         _update(S, t, S.KVCacheFP8(cache.k, cache.v, shared.k_scale, shared.v_scale), [0, 1, 2, 3], cuda)
 
 
+@pytest.mark.parametrize("b", [3, 9, 17])
+def test_a_batch_gives_each_sequence_its_own_bits(cuda, b):
+    """8 kv heads of 3, 9 and 17 sequences: the dims of a head on four, two and one
+    workgroups; the result is the same."""
+    import cuda_decode_attention as A
+    import cuda_decode_small_ops as S
+
+    q, cache = _attend_inputs(S, cuda, b, 16, 8, 2, 1152, seed=b)
+    cache.v.view(torch.uint8)[1, 2, 5, 77, 3] = 0x7F     # row 323 of a sequence that stops before it
+    cache.v.view(torch.uint8)[2, 3, 1, 120, 9] = 0x7F    # row 73 of one that sees it
+    pos = [int(x) for x in torch.randint(0, 1150, (b,), generator=_gen(b))]
+    pos[:3] = [1150, 300, 500]
+    out = _attend_check(q, cache, pos, window=900, sinks=70, what=f"{b} sequences")
+    for i in range(b):
+        one = A.attn_fp8_kv_cache(q[i:i + 1], S.KVCacheFP8(*(t[i:i + 1] for t in cache)), SCALE,
+                                  torch.tensor(pos[i:i + 1], device=cuda), window=900, sinks=70)
+        assert torch.equal(out[i:i + 1].nan_to_num(nan=9e4), one.nan_to_num(nan=9e4)), i
+
+
 def test_one_visible_row_is_returned(cuda):
     import cuda_decode_attention as A
     import cuda_decode_small_ops as S
