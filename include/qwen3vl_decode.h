@@ -309,12 +309,13 @@ int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const
  * S new tokens of each sequence, cos / sin fp16 [B][S][128]; q_out fp16
  * [B][S][Hq][128]; K_rot and V to the rows cache_position[b] + i (int64 [B]; rows
  * outside [0, T) are not written).  q, k, v have batch, token and head strides in
- * elements.  A block that holds rows before cache_position[b] keeps its scale or
+ * elements, multiples of 4, and every operand is 8-byte aligned.  A block that holds rows before cache_position[b] keeps its scale or
  * takes a larger one, and then those rows are scaled down in place (exact but for
  * values that become subnormal); rows behind the last written one keep their
  * bytes, but not their meaning.  Hq is 1 to 64 times Hkv.
  *
- * qd_kv_read_fp8: rows [0, rows) in fp16, k_out and v_out [B][Hkv][rows][128]. */
+ * qd_kv_read_fp8: rows [0, rows) in fp16, k_out and v_out [B][Hkv][rows][128], 16-byte
+ * aligned. */
 int qd_q_rope_kv_update_fp8(const void* q, long q_sb, long q_ss, long q_sh, const void* k, long k_sb, long k_ss,
                             long k_sh, const void* v, long v_sb, long v_ss, long v_sh, const void* q_weight,
                             const void* k_weight, float eps, const void* cos, const void* sin, void* q_out,
@@ -330,7 +331,7 @@ int qd_kv_read_fp8(const void* k_cache, const void* v_cache, const void* k_scale
  * for q head h on kv head h / (Hq / Hkv); query token i stands at
  * p = cache_position[b] + i and sees the rows t <= p, t < T and, with window > 0,
  * t > p - window or t < sinks.  No visible row: zeros.  q fp16 with batch, head and
- * token strides in elements (multiples of 8); out fp16 [B][Sq][Hq][128];
+ * token strides in elements (multiples of 8), out fp16 [B][Sq][Hq][128], both 16-byte aligned;
  * scale > 0.  A NaN in a row that a token does not see has no part in its result.
  * workspace: qd_attention_fp8_workspace_bytes(...) bytes, 16-byte aligned (NULL
  * where that is 0); it holds nothing between calls, but two calls in flight must
