@@ -309,10 +309,11 @@ int qd_block_matmul_fp8(const void* x, const void* x_scale, const void* w, const
  * S new tokens of each sequence, cos / sin fp16 [B][S][128]; q_out fp16
  * [B][S][Hq][128]; K_rot and V to the rows cache_position[b] + i (int64 [B]; rows
  * outside [0, T) are not written).  q, k, v have batch, token and head strides in
- * elements, multiples of 4, and every operand is 8-byte aligned.  A block that holds rows before cache_position[b] keeps its scale or
- * takes a larger one, and then those rows are scaled down in place (exact but for
- * values that become subnormal); rows behind the last written one keep their
- * bytes, but not their meaning.  Hq is 1 to 64 times Hkv.
+ * elements, multiples of 4, and every operand is 8-byte aligned.  A block that holds
+ * rows before cache_position[b] keeps its scale or takes a larger one, and then
+ * those rows are scaled down in place (exact but for values that become subnormal);
+ * rows behind the last written one keep their bytes, but not their meaning.  Hq is 1
+ * to 64 times Hkv.
  *
  * qd_kv_read_fp8: rows [0, rows) in fp16, k_out and v_out [B][Hkv][rows][128], 16-byte
  * aligned. */
