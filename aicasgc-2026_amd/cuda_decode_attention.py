@@ -251,8 +251,8 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
     if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
         raise RuntimeError(f"{name}: window and sinks must lie in [0, 2^31)")
     cp = _positions(name, cache_position, b, dev)
-    qi = _strided_heads(q, 8)
-    out = torch.empty_strided((b, sq, hq, 128), (sq * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
+    qi, *q_at = _strided_heads(q, 8)
+    out = q.new_empty((b, sq, hq, 128))
     need = _fp8_ws_bytes(b, sq, hq, h, t, window, sinks)
     ws = None
     if need:
@@ -264,6 +264,6 @@ def attn_fp8_kv_cache(q, cache, scaling: float, cache_position, window: int = 0,
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             if workspace is not None:
                 workspace[key] = ws
-    _lib.call_on(dev, _lib.entry("qd_attention_fp8"), qi.data_ptr(), *qi.stride()[:3], *where, cp.data_ptr(), scaling, window,
+    _lib.call_on(dev, _lib.entry("qd_attention_fp8"), *q_at, *where, cp.data_ptr(), scaling, window,
                  sinks, out.data_ptr(), b, sq, hq, h, None if ws is None else ws.data_ptr(), need)
     return out

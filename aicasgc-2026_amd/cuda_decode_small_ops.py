@@ -339,21 +339,27 @@ def _positions(name: str, cache_position, b: int, dev: int) -> torch.Tensor:
     return cache_position if cache_position.is_contiguous() else cache_position.contiguous()
 
 
-def _strided_heads(t: torch.Tensor, multiple: int) -> torch.Tensor:
+def _strided_heads(t: torch.Tensor, multiple: int):
     """t [.., .., .., 128] (any order of the first three) itself where its heads can be
-    read in place: contiguous, at strides and an address of whole ``multiple``s."""
+    read in place, contiguous, at strides and an address of whole ``multiple``s, or a
+    copy of it: (tensor to keep, address, the first three strides)."""
     s0, s1, s2, s3 = t.stride()
-    if s3 == 1 and not (s0 | s1 | s2) % multiple and not t.data_ptr() % (2 * multiple):
-        return t
+    ptr = t.data_ptr()
+    if s3 == 1 and not (s0 | s1 | s2) % multiple and not ptr % (2 * multiple):
+        return t, ptr, s0, s1, s2
     t = t.contiguous()
-    return t if not t.data_ptr() % (2 * multiple) else t.clone()
+    if t.data_ptr() % (2 * multiple):
+        t = t.clone()
+    return t, t.data_ptr(), *t.stride()[:3]
 
 
-def _aligned8(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy of it, contiguous at an 8-byte aligned address."""
-    if not t.is_contiguous():
-        return t.contiguous()
-    return t if not t.data_ptr() % 8 else t.clone()
+def _aligned8(t: torch.Tensor):
+    """t, or a copy of it, contiguous at an 8-byte aligned address: (tensor to keep, address)."""
+    ptr = t.data_ptr()
+    if t.is_contiguous() and not ptr % 8:
+        return t, ptr
+    t = t.contiguous() if not t.is_contiguous() else t.clone()
+    return t, t.data_ptr()
 
 
 def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, cos, sin, cache: KVCacheFP8,
@@ -385,11 +391,16 @@ def fused_q_rope_kv_cache_update_fp8(q, k, v, q_weight, k_weight, eps: float, co
     if cos.shape != (b, s, 128) or sin.shape != (b, s, 128):
         raise RuntimeError(f"{name}: cos/sin must be [B, S, 128]")
     cp = _positions(name, cache_position, b, dev)
-    qi, ki, vi = _strided_heads(q, 4), _strided_heads(k, 4), _strided_heads(v, 4)
-    qw, kw, cs, sn = _aligned8(q_weight), _aligned8(k_weight), _aligned8(cos), _aligned8(sin)
-    out = torch.empty_strided((b, s, hq, 128), (s * hq * 128, hq * 128, 128, 1), dtype=torch.float16, device=q.device)
-    _lib.call_on(dev, _lib.entry("qd_q_rope_kv_update_fp8"), qi.data_ptr(), *qi.stride()[:3], ki.data_ptr(), *ki.stride()[:3],
-                 vi.data_ptr(), *vi.stride()[:3], qw.data_ptr(), kw.data_ptr(), eps, cs.data_ptr(), sn.data_ptr(),
+    # (the copies, where there are any, live until the launch)
+    qi, *q_at = _strided_heads(q, 4)
+    ki, *k_at = _strided_heads(k, 4)
+    vi, *v_at = _strided_heads(v, 4)
+    qw, qw_at = _aligned8(q_weight)
+    kw, kw_at = _aligned8(k_weight)
+    cs, cs_at = _aligned8(cos)
+    sn, sn_at = _aligned8(sin)
+    out = _EMPTY_LIKE(q, memory_format=torch.contiguous_format)
+    _lib.call_on(dev, _lib.entry("qd_q_rope_kv_update_fp8"), *q_at, *k_at, *v_at, qw_at, kw_at, eps, cs_at, sn_at,
                  out.data_ptr(), *where, cp.data_ptr(), b, s, hq, h)
     return out
 
